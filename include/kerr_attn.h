@@ -391,6 +391,95 @@ int kattn_block_fwd(kattn_ctx* ctx, kattn_block* blk, const kattn_block_params* 
 int kattn_block_bwd(kattn_ctx* ctx, kattn_block* blk, const float* dh_out, float* dh,
                     const kattn_block_grads* grads, int accumulate, void* stream);
 
+/* ---- Serving: packed prompts, an 8-bit paged cache, attention over it -------
+ * Answering with a trained model: prompts of different lengths run together,
+ * their keys and values stay in a cache, and each further step attends one
+ * new token of every sequence, a few, or a tree of drafted ones over it.  The
+ * reference answers by running the whole context again for every token
+ * (src/model.rs:364-431); it has no cache, no packing and one key head per
+ * query head, so these calls have no counterpart of their own there.
+ *
+ * Rows.  The new tokens of S sequences are packed rows: sequence s owns rows
+ * cu[s] .. cu[s+1]-1 of q, k, v and o ([rows][heads*d], a row stride in
+ * elements each), where cu is S+1 ascending int32 on the device, cu[0] >= 0,
+ * cu[S] <= N.  A sequence may have no rows.  N is the rows the arrays hold:
+ * rows before cu[0] and behind cu[S] are neither read nor written, so arrays
+ * padded to a fixed N (a captured graph) are fine.  Query heads are grouped:
+ * query head h uses key head h / (H / Hkv), H a multiple of Hkv.  lse is
+ * [H][N].  Lengths, tables and pages live on the device; the calls read them
+ * there and never synchronise the host.
+ *
+ * Types.  dtype names the element type of q, k, v and o: scores, softmax
+ * statistics and sums are formed in f32 (in bf16 hi/lo or f16 hi/lo products,
+ * about 1e-5, for KATTN_F32), and outputs are rounded once.  Device pointers
+ * are 16-byte aligned and row strides a multiple of 16 bytes; int32 arrays
+ * and lse 4-byte, tree 8-byte aligned.  d is 32, 64 or 128.
+ *
+ * A row that sees nothing has o = 0 and lse = -inf.  A NaN or an infinity in
+ * a sequence's rows reaches the outputs of that sequence only. */
+enum { KATTN_F32 = 0, KATTN_BF16 = 1, KATTN_F16 = 2 };
+
+/* Causal attention of packed sequences.  Sequence s has nq = cu_q[s+1] -
+ * cu_q[s] query rows and nk = cu_k[s+1] - cu_k[s] key rows; the last query row
+ * sees all keys, the one before all but the last, and so on: row i sees keys j <=
+ * i + nk - nq (every key when causal == 0).  So nk == nq is a prompt, nk > nq a
+ * prompt's next chunk behind its earlier context (kattn_cache_read gives its
+ * keys and values), and with nk < nq the first rows see nothing. */
+int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const void* k, const void* v, long ld_kv,
+                     void* o, long ld_o, float* lse, const int* cu_q, const int* cu_k, int S, int Nq, int Nk, int H,
+                     int Hkv, int d, float scale, int causal, void* stream);
+
+/* How a cache holds a token's row of d values of one key head: 8-bit codes
+ * and one f32 scale, value = code * scale.  With m the row's largest
+ * magnitude and L the largest code (127, or e4m3's 448), scale = m / L and
+ * code = x * (L / m), each quotient rounded to f32 and the product rounded
+ * once, to the nearest code, ties to even.  A row with m < 2^-100 is held as zeros; one
+ * with an infinity or a NaN reads back as NaN throughout. */
+enum { KATTN_CACHE_INT8 = 0, KATTN_CACHE_E4M3 = 1 };
+
+/* A paged cache in caller-owned device memory (16-byte aligned codes):
+ *   k, v              [n_pages][n_kv_head][page_size][d] codes
+ *   k_scale, v_scale  [n_pages][n_kv_head][page_size]
+ * page_size is 16, 32, 64, 128 or 256.  Position p of sequence s is at place
+ * p % page_size of page table[s][p / page_size] (int32, row stride ld_table,
+ * max_pages entries used).  kv_len[s] (int32) is the sequence's length with
+ * its new tokens: its n = cu[s+1] - cu[s] rows are the positions kv_len[s] - n
+ * .. kv_len[s] - 1.  Positions that are negative, past max_pages pages, or on a page
+ * outside 0 .. n_pages-1 do not exist: nothing is written there, they
+ * read as zeros, and no row sees them. */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int n_pages, page_size, n_kv_head, d, format;
+} kattn_kv_cache;
+
+/* Quantises the new tokens' k and v rows ([N][n_kv_head*d]) into the cache.
+ * Two rows at one place (a page shared by two sequences' new tokens) race. */
+int kattn_cache_append(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, const void* k, const void* v,
+                       long ld_kv, const int* cu, const int* kv_len, const int* table, long ld_table, int max_pages,
+                       int S, int N, void* stream);
+
+/* Reads rows back from the cache: row cu[s] + i receives the values of
+ * position kv_len[s] - n + i, rounded once to dtype.  cu = the running sum of
+ * kv_len reads whole sequences. */
+int kattn_cache_read(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, void* k, void* v, long ld_kv,
+                     const int* cu, const int* kv_len, const int* table, long ld_table, int max_pages, int S, int N,
+                     void* stream);
+
+/* Attention of the new tokens over the cache, which already holds their own
+ * keys and values (kattn_cache_append comes first).  A row sees every
+ * position before the sequence's new tokens and, of the new ones, those up to
+ * its own (tree == NULL), or, with a tree of drafted tokens, the j-th where bit
+ * j of tree[row] is set: its ancestors and, as a rule, itself.  tree is [N];
+ * drafted tokens past a sequence's 64th have no bit and are seen by no row.
+ * Workspace for the parts of long sequences comes from the context's pool;
+ * parts are joined in a fixed order, so the same inputs give the same bits. */
+int kattn_fwd_cached(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, const void* q, long ld_q, void* o,
+                     long ld_o, float* lse, const int* cu, const int* kv_len, const int* table, long ld_table,
+                     int max_pages, const unsigned long long* tree, int S, int N, int H, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

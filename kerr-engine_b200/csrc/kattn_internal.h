@@ -34,6 +34,8 @@ struct kattn_ctx {
 
 namespace kattn_abi {
 
+extern thread_local int g_last_launches;  // kattn_last_launch_count of this thread
+
 // Records a formatted message for kattn_last_error and returns `status`.
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // KATTN_ERR_CUDA (KATTN_ERR_OUT_OF_MEMORY for an allocation failure) with

@@ -165,4 +165,55 @@ ProjStatus kode_backward(cudaStream_t s, int num_sms, const float* dy, long ld_d
                          float* d_gamma_raw, float* d_omega, float* d_alpha_beta, int M, int nb, int n_steps,
                          int accumulate, float* part, int part_rows, int* launches);
 
+// ---- Serving (include/kerr_attn.h; arguments checked there).  `dtype` is a
+// KATTN_F32 / _BF16 / _F16 value; sequence s owns rows cu[s] .. cu[s+1]-1.
+struct PackedArgs {
+    int dtype;
+    const void* q;
+    long ld_q;
+    const void* k;
+    const void* v;
+    long ld_kv;
+    void* o;
+    long ld_o;
+    float* lse;
+    const int* cu_q;
+    const int* cu_k;
+    int S, Nq, Nk, H, Hkv, d;
+    float scale;
+    int causal;
+    int* status = nullptr;
+    unsigned long long wait_ns = 1000000000ull;
+};
+ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
+
+// A batch's place in a paged cache.
+struct CacheArgs {
+    kattn_kv_cache c;
+    const int* cu;
+    const int* kv_len;
+    const int* table;
+    long ld_table;
+    int max_pages, S, N;
+};
+// k and v: the rows to hold (append) or to fill (read).
+ProjStatus cache_append(const CacheArgs& a, int dtype, const void* k, const void* v, long ld, int num_sms,
+                        cudaStream_t s, int* launches);
+ProjStatus cache_read(const CacheArgs& a, int dtype, void* k, void* v, long ld, int num_sms, cudaStream_t s,
+                      int* launches);
+
+struct CachedArgs {
+    CacheArgs cache;
+    int dtype;
+    const void* q;
+    long ld_q;
+    void* o;
+    long ld_o;
+    float* lse;
+    const unsigned long long* tree;
+    int H;
+    float scale;
+};
+ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
+
 }  // namespace kattn

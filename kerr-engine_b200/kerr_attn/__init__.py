@@ -30,6 +30,11 @@ KATTN_ERR_CUDA = 5
 KATTN_ERR_OUT_OF_MEMORY = 6
 KATTN_ERR_DEVICE_TIMEOUT = 7
 
+# How a KVCache holds its rows (kattn_kv_cache.format).
+CACHE_INT8 = 0
+CACHE_E4M3 = 1
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
 PATH_AUTO = 0
 PATH_FFMA = 1
 PATH_TENSOR = 2
@@ -46,6 +51,7 @@ EXPORTED_SYMBOLS = (
     "kattn_layernorm_fwd", "kattn_layernorm_bwd",
     "kattn_kerr_ode_fwd", "kattn_kerr_ode_bwd", "kattn_kerr_ode_fwd_host", "kattn_kerr_ode_bwd_host",
     "kattn_block_create", "kattn_block_destroy", "kattn_block_fwd", "kattn_block_bwd",
+    "kattn_fwd_packed", "kattn_cache_append", "kattn_cache_read", "kattn_fwd_cached",
 )
 
 # Widest row kattn_layernorm_fwd / _bwd accept (KATTN_LN_MAX_N).
@@ -149,6 +155,16 @@ def lib():
     L.kattn_kerr_ode_fwd_host.restype = _i
     L.kattn_kerr_ode_bwd_host.argtypes = [_p, _p, _l, _p, _l, _p, _p, _fl, _fl, _p, _l, _p, _p, _p, _i, _i, _i, _i]
     L.kattn_kerr_ode_bwd_host.restype = _i
+    cache_args = [_p, ctypes.POINTER(KVCacheTable), _i, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _p]
+    L.kattn_fwd_packed.argtypes = [_p, _i, _p, _l, _p, _p, _l, _p, _l, _p, _p, _p] + [_i] * 6 + [_fl, _i, _p]
+    L.kattn_fwd_packed.restype = _i
+    L.kattn_cache_append.argtypes = cache_args
+    L.kattn_cache_append.restype = _i
+    L.kattn_cache_read.argtypes = cache_args
+    L.kattn_cache_read.restype = _i
+    L.kattn_fwd_cached.argtypes = [_p, ctypes.POINTER(KVCacheTable), _i, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _p,
+                                   _i, _i, _i, _fl, _p]
+    L.kattn_fwd_cached.restype = _i
     _lib = L
     return L
 
@@ -684,3 +700,211 @@ class Block:
             self.close()
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------- serving
+# Packed prompts, the 8-bit paged cache and attention over it
+# (include/kerr_attn.h, kattn_fwd_packed / kattn_cache_* / kattn_fwd_cached).
+# q / o are [N, n_head*d], k / v [N, n_kv_head*d] CUDA views of one type
+# (float32, bfloat16 or float16) with unit inner stride; cu, kv_len and tables
+# are int32 CUDA tensors.
+
+class KVCacheTable(ctypes.Structure):
+    """kattn_kv_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_kv_head", ctypes.c_int), ("d", ctypes.c_int), ("format", ctypes.c_int)]
+
+
+class KVCache:
+    """Pages of 8-bit keys and values (kattn_kv_cache): k, v are int8 or uint8
+    [n_pages, n_kv_head, page_size, d], k_scale, v_scale float32 [n_pages,
+    n_kv_head, page_size], contiguous CUDA tensors that the object keeps."""
+
+    def __init__(self, k, v, k_scale, v_scale, fmt: int = CACHE_INT8):
+        import torch
+
+        if k.dim() != 4:
+            raise ValueError("k must be [n_pages, n_kv_head, page_size, d]")
+        for t, name, shape, kinds in ((k, "k", k.shape, (torch.int8, torch.uint8)),
+                                      (v, "v", k.shape, (torch.int8, torch.uint8)),
+                                      (k_scale, "k_scale", k.shape[:3], (torch.float32,)),
+                                      (v_scale, "v_scale", k.shape[:3], (torch.float32,))):
+            if t.dtype not in kinds or not t.is_cuda or not t.is_contiguous() or t.shape != shape:
+                raise ValueError(f"{name} must be a contiguous CUDA tensor of shape {tuple(shape)} and type {kinds}")
+            if t.device != k.device:
+                raise ValueError(f"{name} is on another device than k")
+        self.k, self.v, self.k_scale, self.v_scale, self.format = k, v, k_scale, v_scale, int(fmt)
+        self.n_pages, self.n_kv_head, self.page_size, self.d = k.shape
+        self.device = k.device
+        self._table = KVCacheTable(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.n_pages,
+                                   self.page_size, self.n_kv_head, self.d, self.format)
+        self._ref = ctypes.byref(self._table)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv_head: int, d: int, fmt: int = CACHE_INT8, device="cuda"):
+        """A cache whose pages hold zeros."""
+        import torch
+
+        shape = (n_pages, n_kv_head, page_size, d)
+        return cls(torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape[:3], device=device), torch.zeros(shape[:3], device=device), fmt)
+
+
+_dtype_codes = None
+
+
+def _dtype_code(t, name):
+    """KATTN_F32 / KATTN_BF16 / KATTN_F16."""
+    global _dtype_codes
+    if _dtype_codes is None:
+        import torch
+
+        _dtype_codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    code = _dtype_codes.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16")
+    return code
+
+
+def _packed(t, name, like, cols):
+    """(pointer, row stride) of a [rows, cols] view of `like`'s type and device."""
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not {like.device}")
+    if t.dim() != 2 or t.shape[1] != cols:
+        raise ValueError(f"{name} must be [rows, {cols}]")
+    if t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit inner stride")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols))
+
+
+def _ints(t, name, n, device):
+    if t.dtype != _int32() or not t.is_contiguous() or t.device != device or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def _int32():
+    import torch
+    return torch.int32
+
+
+def _on(ctx, t, name):
+    """The tensor's device, which has to be the context's."""
+    device = t.device
+    if device.type != "cuda" or device.index != ctx.device:
+        raise ValueError(f"{name} is on {device}, the context on cuda:{ctx.device}")
+    return device
+
+
+def _sums(lse, n_head, n, device):
+    if lse.dtype != _f32() or not lse.is_contiguous() or tuple(lse.shape) != (n_head, n) or lse.device != device:
+        raise ValueError(f"lse must be a contiguous float32 tensor of shape ({n_head}, {n}) on {device}")
+    return lse.data_ptr()
+
+
+def _pages(cache, cu, kv_len, table, device):
+    """The arguments that place a batch in the cache."""
+    if cache.device != device:
+        raise ValueError(f"the cache is on {cache.device}, not {device}")
+    S = kv_len.shape[0]
+    if table.dtype != _int32() or table.device != device or table.dim() != 2 or table.shape[0] != S:
+        raise ValueError(f"table must be an int32 [{S}, pages] tensor on {device}")
+    pages = table.shape[1]
+    if pages > 1 and table.stride(1) != 1:
+        raise ValueError("table must have unit inner stride")
+    return (_ints(cu, "cu", S + 1, device), _ints(kv_len, "kv_len", S, device), table.data_ptr(),
+            max(table.stride(0), pages), pages), S
+
+
+def fwd_packed(ctx: Context, q, k, v, o, lse, cu_q, cu_k, n_head: int, n_kv_head: int | None = None,
+               causal: bool = True, scale: float | None = None, stream=None) -> int:
+    """Causal attention of packed sequences with grouped heads: rows cu_q[s] ..
+    cu_q[s+1]-1 of q, o [Nq, n_head*d] over rows cu_k[s] .. cu_k[s+1]-1 of k, v
+    [Nk, n_kv_head*d], the last query row seeing all keys; lse [n_head, Nq].
+    Returns kernels launched."""
+    kv = n_head if n_kv_head is None else n_kv_head
+    if n_head <= 0 or kv <= 0:
+        raise ValueError("head counts must be positive")
+    device = _on(ctx, q, "q")
+    N, C = q.shape
+    d = C // n_head
+    dtype = _dtype_code(q, "q")
+    pq, ldq = _packed(q, "q", q, n_head * d)
+    pk, ldk = _packed(k, "k", q, kv * d)
+    pv, ldv = _packed(v, "v", q, kv * d)
+    po, ldo = _packed(o, "o", q, C)
+    if k.shape[0] != v.shape[0] or o.shape[0] != N:
+        raise ValueError("q and o, k and v must have the same rows")
+    if ldk != ldv:
+        raise ValueError("k, v must share one row stride")
+    S = cu_q.shape[0] - 1
+    st = lib().kattn_fwd_packed(ctx.handle, dtype, pq, ldq, pk, pv, ldk, po, ldo, _sums(lse, n_head, N, device),
+                                _ints(cu_q, "cu_q", S + 1, device), _ints(cu_k, "cu_k", S + 1, device), S, N,
+                                k.shape[0], n_head, kv, d, 1.0 / math.sqrt(d) if scale is None else scale,
+                                1 if causal else 0, _stream_ptr(stream, device))
+    _check(st, "kattn_fwd_packed")
+    return last_launch_count()
+
+
+def cache_append(ctx: Context, cache: KVCache, k, v, cu, kv_len, table, stream=None) -> int:
+    """Quantises the rows of k, v [N, n_kv_head*d] into the cache: sequence s's
+    rows cu[s] .. cu[s+1]-1 are its last positions before kv_len[s], on the
+    pages table[s].  Returns kernels launched."""
+    return _cache_rows("kattn_cache_append", ctx, cache, k, v, cu, kv_len, table, stream)
+
+
+def cache_read(ctx: Context, cache: KVCache, k, v, cu, kv_len, table, stream=None) -> int:
+    """Fills k, v [N, n_kv_head*d] with the values that the cache holds for the
+    positions that :func:`cache_append` would write.  Returns kernels launched."""
+    return _cache_rows("kattn_cache_read", ctx, cache, k, v, cu, kv_len, table, stream)
+
+
+def _cache_rows(what, ctx, cache, k, v, cu, kv_len, table, stream):
+    device = _on(ctx, k, "k")
+    dtype = _dtype_code(k, "k")
+    cols = cache.n_kv_head * cache.d
+    pk, ldk = _packed(k, "k", k, cols)
+    pv, ldv = _packed(v, "v", k, cols)
+    if ldk != ldv or k.shape[0] != v.shape[0]:
+        raise ValueError("k, v must share their rows and one row stride")
+    where, S = _pages(cache, cu, kv_len, table, device)
+    st = getattr(lib(), what)(ctx.handle, cache._ref, dtype, pk, pv, ldk, *where, S, k.shape[0],
+                              _stream_ptr(stream, device))
+    _check(st, what)
+    return last_launch_count()
+
+
+def fwd_cached(ctx: Context, cache: KVCache, q, o, lse, cu, kv_len, table, n_head: int, tree=None,
+               scale: float | None = None, stream=None) -> int:
+    """Attention of each sequence's new tokens (rows cu[s] .. cu[s+1]-1 of q, o
+    [N, n_head*d]) over its cache, which holds them already; tree (int64 [N])
+    gives, as bits, the drafted tokens that each row sees (None: those up to its own).
+    lse [n_head, N].  Returns kernels launched."""
+    device = _on(ctx, q, "q")
+    N = q.shape[0]
+    d = cache.d
+    dtype = _dtype_code(q, "q")
+    pq, ldq = _packed(q, "q", q, n_head * d)
+    po, ldo = _packed(o, "o", q, n_head * d)
+    if o.shape[0] != N:
+        raise ValueError("q and o must have the same rows")
+    where, S = _pages(cache, cu, kv_len, table, device)
+    bits = None
+    if tree is not None:
+        if tree.dtype != _int64() or not tree.is_contiguous() or tuple(tree.shape) != (N,) or tree.device != device:
+            raise ValueError(f"tree must be a contiguous int64 tensor of {N} elements on {device}")
+        bits = tree.data_ptr()
+    st = lib().kattn_fwd_cached(ctx.handle, cache._ref, dtype, pq, ldq, po, ldo, _sums(lse, n_head, N, device),
+                                *where, bits, S, N, n_head, 1.0 / math.sqrt(d) if scale is None else scale,
+                                _stream_ptr(stream, device))
+    _check(st, "kattn_fwd_cached")
+    return last_launch_count()
+
+
+def _int64():
+    import torch
+    return torch.int64
