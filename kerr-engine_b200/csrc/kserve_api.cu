@@ -120,6 +120,8 @@ int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const 
     KATTN_TRY(check_heads(H, Hkv, d));
     KATTN_TRY(check_counts(S, Nq));
     if (Nk < 0) return fail(KATTN_ERR_INVALID_ARGUMENT, "negative size (Nk=%d)", Nk);
+    if (static_cast<long>(Nq) * H > INT_MAX || Nk > INT_MAX - 256 || static_cast<long>(S) * Hkv > INT_MAX / 2)
+        return fail(KATTN_ERR_INVALID_ARGUMENT, "problem too large (Nq=%d H=%d Nk=%d S=%d)", Nq, H, Nk, S);
     if (!std::isfinite(scale)) return fail(KATTN_ERR_INVALID_ARGUMENT, "scale is not finite");
     if (causal != 0 && causal != 1) return fail(KATTN_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
     if (S == 0 || Nq == 0) return ok_with_launches(0);
@@ -138,7 +140,7 @@ int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const 
                               scale, causal, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed)};
     int launches = 0;
     const kattn::ProjStatus st =
-        kattn::packed_forward(a, ctx->num_sms, ctx->pool, static_cast<cudaStream_t>(stream), &launches);
+        kattn::packed_forward(a, ctx->num_sms, static_cast<cudaStream_t>(stream), &launches);
     return result(st, launches);
 }
 

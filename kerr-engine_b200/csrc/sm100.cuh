@@ -291,6 +291,11 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, int a_mn, int b_
            | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
 }
 
+// The same for f16 A and B.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn, int b_mn) {
+    return idesc_bf16(M, N, a_mn, b_mn) & ~((1u << 7) | (1u << 10));
+}
+
 // D[tmem] (+)= A[smem] * B[smem]
 __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -329,6 +334,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float even, float odd) {
 }
 __device__ __forceinline__ float bf16_lo_f(uint32_t packed) { return __uint_as_float(packed << 16); }
 __device__ __forceinline__ float bf16_hi_f(uint32_t packed) { return __uint_as_float(packed & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t pack_f16(float even, float odd) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(odd), "f"(even));
+    return r;
+}
+
+// Moves registers between the warpgroups of a CTA; every warp of a warpgroup
+// executes it.  The sum over the warpgroups stays within the launch's total.
+template <int REGS>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
 
 // ---------------------------------------------------------------- 256-bit global access
 // 32 bytes of read-only global memory in one 256-bit load (sm_100); p must
