@@ -213,6 +213,8 @@ struct CachedArgs {
     const unsigned long long* tree;
     int H;
     float scale;
+    int* status = nullptr;
+    unsigned long long wait_ns = 1000000000ull;
 };
 ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
 

@@ -36,7 +36,7 @@ __device__ __forceinline__ void find_places(const CacheArgs& a, int page_shift, 
                 const int2 rows = seq_rows(a.cu, s, a.N);
                 if (r < rows.y) {
                     mine = true;
-                    const int p = __ldg(a.kv_len + s) - (rows.y - r);
+                    const int p = max(__ldg(a.kv_len + s), 0) - (rows.y - r);
                     const int page = page_of(a, page_shift, s, p);
                     if (page >= 0)
                         at = (static_cast<long>(page) * a.c.n_kv_head << page_shift) + (p & (a.c.page_size - 1));

@@ -5,92 +5,890 @@
 //
 // with the codes kc, vc and scales ks, vs of position j, for the positions
 // that row i sees: those before the new tokens, and of the new ones the tree's.
+//
+// What bounds it is the cache: each byte is read once for a handful of rows,
+// so the work is to keep enough copies in flight and to turn codes into
+// MMA operands with few instructions.
+//
+// Rows.  The G query heads of a key head share its positions: a sequence's n
+// tokens are n * G rows, in row tiles of 16 * MT, the m of mma.m16n8k16.
+//
+// Split.  The (sequence, key head, row tile) items and their tiles of 64 positions
+// are one line of work, cut into as many equal parts as there are CTAs
+// (two to an SM), whatever the lengths; an item cut by a border leaves parts
+// (row maxima, sums, O) in a workspace, which cached_join adds in order.
+//
+// Operands.  Codes are exact in f16 (int8 as they are, e4m3 times 2^-8), so
+// only q and the weights are rounded: q to f16 after a power of two per row has
+// brought its largest element near 2^13 (exact for bf16 and f16 but for elements 2^-37
+// of it; f32 as a hi / lo pair), the weights p_j vs_j to f16 after a power of two
+// per warp (f32: as a pair).  The scale ks_j multiplies the score.
+//
+// A warp takes 16 of a tile's 64 positions.  Its lanes read whole 16-byte chunks
+// of codes: the order of d in the first product is free (q is permuted
+// alike), and in the second a lane's chunk spreads over 16 of the n8 tiles, which
+// leaves it 32 neighbouring columns of O.  tau() orders a tile's positions so that
+// both reads meet no bank twice under the copy's swizzle.
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
+#include <cuda.h>
+
 #include "kserve.cuh"
+#include "sm100.cuh"
+#include "tma_map.h"
 
 namespace kattn {
 
 namespace {
 
 using namespace serve;
+using namespace sm100;
 
-// One warp per (row, query head): a lane holds D / 32 columns, positions one by one.
-template <class T, int D, int FORMAT>
-__global__ void __launch_bounds__(128) cached_rows(CachedArgs a, int page_shift) {
-    constexpr int E = D / 32;
-    pdl_enter();
-    const CacheArgs& b = a.cache;
-    const int lane = threadIdx.x & 31;
-    const long units = static_cast<long>(b.N) * a.H;
-    const float c = a.scale * kLog2e;
-    for (long u = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5); u < units; u += 4L * gridDim.x) {
-        const int r = static_cast<int>(u / a.H), h = static_cast<int>(u % a.H);
-        const int s = seq_of_row(b.cu, b.S, r);
-        if (s < 0) continue;
-        const int2 rows = seq_rows(b.cu, s, b.N);
-        if (r >= rows.y) continue;
-        const int len = __ldg(b.kv_len + s), base = len - (rows.y - rows.x);
-        const unsigned long long bits = a.tree ? __ldg(a.tree + r) : 0;
-        const int hk = h / (a.H / b.c.n_kv_head);
-        const T* q = static_cast<const T*>(a.q) + static_cast<long>(r) * a.ld_q + h * D + lane * E;
-        float x[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = to_f32(q[i]), acc[i] = 0.f;
-        for (int j = 0; j < len; ++j) {
-            if (j >= base) {
-                const int t = j - base;
-                if (a.tree ? t >= 64 || !((bits >> t) & 1) : t > r - rows.x) continue;
-            }
-            const int page = page_of(b, page_shift, s, j);
-            if (page < 0) continue;
-            const long row = ((static_cast<long>(page) * b.c.n_kv_head + hk) << page_shift) + (j & (b.c.page_size - 1));
-            const uint8_t* k = static_cast<const uint8_t*>(b.c.k) + row * D + lane * E;
-            const uint8_t* v = static_cast<const uint8_t*>(b.c.v) + row * D + lane * E;
-            float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < E; ++i) dot = fmaf(x[i], code_value<FORMAT>(k[i]), dot);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            const float y = dot * b.c.k_scale[row] * c, m2 = fmaxf(m, y);
-            const float keep = ex2(m - m2), p = ex2(y - m2);
-            m = m2;
-            l = fmaf(l, keep, p);
-            const float w = p * b.c.v_scale[row];
-#pragma unroll
-            for (int i = 0; i < E; ++i) acc[i] = fmaf(w, code_value<FORMAT>(v[i]), acc[i] * keep);
-        }
-        T* o = static_cast<T*>(a.o) + static_cast<long>(r) * a.ld_o + h * D + lane * E;
-        const bool any = l != 0.f;
-        const float inv = any ? 1.f / l : 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = from_f32<T>(acc[i] * inv);
-        if (lane == 0) a.lse[static_cast<long>(h) * b.N + r] = any ? (m + log2f(l)) * kLn2 : -INFINITY;
+constexpr int TK = 64;     // positions of a tile
+constexpr int WARPS = 4;   // computing warps, 16 positions of a tile each
+constexpr int N_THREADS = 32 * (WARPS + 1);
+constexpr float RAISE = 8.f;         // a row's reference is raised when its maximum passes it by 2^8
+constexpr float W_UP = 128.f;        // weights are held times 2^7: at most 2^15 with RAISE, far from f16's subnormals
+
+// A part's place in the line of work, and what joins it.
+struct Join {
+    int first_cta;  // holds the item's first part; -1: this CTA ends no item that others began
+    int row0, rows; // the item's first row among the sequence's n * G, and how many
+    int q0, hk;
+};
+
+struct Params {
+    CUtensorMap tk, tv;
+    CachedArgs a;
+    int page_shift, G;
+    float* part_o;   // [2 * CTAs][rows][D]: a CTA's part that began before it (0) or begins in it (1)
+    float2* part_ml; // [2 * CTAs][rows]
+    Join* joins;     // [CTAs]
+};
+
+template <int D, int MT, bool SPLIT>
+struct Cfg {
+    static constexpr int MR = 16 * MT;
+    static constexpr int KS = D / 16;                      // k steps of the first product
+    static constexpr bool Q_SMEM = MT > 1;                 // q in shared memory (registers are O's)
+    static constexpr int Q_WORDS = Q_SMEM ? KS * MT * (SPLIT ? 2 : 1) * 32 : 1;
+    static constexpr int STAGES = MT > 1 && D == 128 ? 3 : 4;
+};
+
+template <int D, int MT, bool SPLIT>
+struct Smem {
+    using C = Cfg<D, MT, SPLIT>;
+    alignas(1024) uint8_t k[C::STAGES][TK * D];
+    alignas(1024) uint8_t v[C::STAGES][TK * D];
+    alignas(16) float ks[C::STAGES][TK];
+    alignas(16) float vs[C::STAGES][TK];
+    alignas(16) uint4 q[C::Q_WORDS];
+    alignas(16) float4 o[2][C::MR * D / 4];  // exchange of two warps' O
+    float2 ml[WARPS][C::MR];
+    float unit[WARPS];
+    uint32_t valid[C::STAGES];  // a bit for each 16 positions: they exist
+    uint64_t full[C::STAGES], empty[C::STAGES];
+};
+
+// The position, of 8, behind column n = 2t + b of an n8 tile.
+template <int D>
+__device__ __forceinline__ int tau(int n) {
+    const int b = n & 1, lo = (n >> 1) & 1, hi = n >> 2;
+    if constexpr (D == 128) return ((b ^ hi) << 2) | (lo << 1) | hi;
+    else if constexpr (D == 64) return (hi << 2) | (lo << 1) | (b ^ lo);
+    else return (hi << 2) | ((b ^ hi) << 1) | lo;
+}
+
+// Byte offset of the 16-byte chunk ch of row r in a tile as the copy swizzles it.
+template <int D>
+__device__ __forceinline__ int chunk_at(int r, int ch) {
+    if constexpr (D == 128) return r * 128 + ((ch ^ (r & 7)) << 4);
+    else if constexpr (D == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
+    else return r * 32 + ((ch ^ ((r >> 2) & 1)) << 4);
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// Codes as f16 pairs.  int8: code + 128 under 1024's exponent is 1152 + code.
+// e4m3: its exponent and mantissa under f16's, the number times 2^-8.  Codes
+// arrive through prepare(), one word of four.
+template <int FORMAT>
+struct Codes {
+    static constexpr float VALUE = FORMAT == KATTN_CACHE_INT8 ? 1.f : 256.f;  // of a converted code's one
+    static __device__ __forceinline__ uint32_t prepare(uint32_t w) {
+        return FORMAT == KATTN_CACHE_INT8 ? w ^ 0x80808080u : w;
     }
+    // Bytes I and J of w (a prepared word, or two of them interleaved).
+    template <int I, int J>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+        if constexpr (FORMAT == KATTN_CACHE_INT8) {
+            return sub2(prmt(w, 0x64646464u, 0x4040u | I | (J << 8)), 0x64806480u);
+        } else {
+            const uint32_t x = prmt(w, 0u, 0x0404u | (I << 4) | (J << 12));
+            return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u);
+        }
+    }
+};
+
+// ---------------------------------------------------------------- the line of work
+struct Piece {
+    int s, q0, n, len;   // sequence, its first row, rows and length
+    int hk, row0;        // key head, first row of the row tile
+    int t0, t1, tiles;   // its tiles t0 .. t1-1 of the item's
+    long start;          // the item's first tile in the line
+};
+
+template <int MR>
+struct Line {
+    const CachedArgs& a;
+    int G, lane, capacity;  // positions that the tables hold
+    long at, end, total;    // the CTA's tiles, all tiles
+    int ctas;
+    int s, row_tiles, tiles, q0, n, len;  // current sequence
+    long base;                            // its first tile
+
+    __device__ __forceinline__ long load(int i) {  // sequence i's tiles
+        const int2 r = seq_rows(a.cache.cu, i, a.cache.N);
+        q0 = r.x;
+        n = r.y - r.x;
+        len = min(max(__ldg(a.cache.kv_len + i), 0), capacity);
+        row_tiles = (n * G + MR - 1) / MR;
+        tiles = max(1, (len + TK - 1) / TK);
+        return static_cast<long>(row_tiles) * a.cache.c.n_kv_head * tiles;
+    }
+    // Finds the CTA's part; whole warps.
+    __device__ __forceinline__ bool start(int cta, int grid) {
+        long sum = 0;
+        for (int i = lane; i < a.cache.S; i += 32) sum += load(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        total = sum;
+        ctas = static_cast<int>(min(static_cast<long>(grid), total));
+        if (cta >= ctas) return false;
+        at = cta * total / ctas;
+        end = (cta + 1) * total / ctas;
+        long before = 0;
+        for (int i0 = 0;; i0 += 32) {
+            const int i = i0 + lane;
+            const long mine = i < a.cache.S ? load(i) : 0;
+            long run = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long x = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += x;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + run > at);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                s = i0 + src;
+                base = before + __shfl_sync(0xffffffffu, run - mine, src);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, run, 31);
+        }
+        load(s);
+        return true;
+    }
+    // The next piece of the CTA's part; false: none is left.
+    __device__ __forceinline__ bool next(Piece& p) {
+        if (at >= end) return false;
+        long mine = static_cast<long>(row_tiles) * a.cache.c.n_kv_head * tiles;
+        while (at >= base + mine) {
+            base += mine;
+            mine = load(++s);
+        }
+        const int item = static_cast<int>((at - base) / tiles);
+        p.s = s;
+        p.q0 = q0;
+        p.n = n;
+        p.len = len;
+        p.hk = item / row_tiles;
+        p.row0 = (item % row_tiles) * MR;
+        p.tiles = tiles;
+        p.start = base + static_cast<long>(item) * tiles;
+        p.t0 = static_cast<int>(at - p.start);
+        p.t1 = static_cast<int>(min(static_cast<long>(tiles), end - p.start));
+        at = p.start + p.t1;
+        return true;
+    }
+    // The CTA that holds the line's tile g.
+    __device__ __forceinline__ int owner(long g) const { return static_cast<int>(((g + 1) * ctas + total - 1) / total) - 1; }
+};
+
+// ---------------------------------------------------------------- rows
+// Four neighbouring elements of q (16-byte rows, so 8-byte pieces are aligned).
+__device__ __forceinline__ float4 load_q4(const CachedArgs& a, long i) {
+    if (a.dtype == KATTN_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + i));
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + i));
+    if (a.dtype == KATTN_BF16)
+        return make_float4(bf16_lo_f(w.x), bf16_hi_f(w.x), bf16_lo_f(w.y), bf16_hi_f(w.y));
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+
+// N (a multiple of 4) neighbouring outputs, rounded once.
+template <int N>
+__device__ __forceinline__ void store_out(const CachedArgs& a, long i, const float (&x)[N]) {
+    if (a.dtype == KATTN_F32) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.o) + i);
+#pragma unroll
+        for (int u = 0; u < N / 4; ++u) p[u] = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+    } else {
+        uint2* p = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + i);
+#pragma unroll
+        for (int u = 0; u < N / 4; ++u)
+            p[u] = a.dtype == KATTN_BF16
+                       ? make_uint2(pack_bf16(x[4 * u], x[4 * u + 1]), pack_bf16(x[4 * u + 2], x[4 * u + 3]))
+                       : make_uint2(pack_f16(x[4 * u], x[4 * u + 1]), pack_f16(x[4 * u + 2], x[4 * u + 3]));
+    }
+}
+
+// ---------------------------------------------------------------- kernel
+template <int D, int FORMAT, int MT, bool SPLIT>
+__global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant__ Params p) {
+    using C = Cfg<D, MT, SPLIT>;
+    using Code = Codes<FORMAT>;
+    constexpr int MR = C::MR, KS = C::KS, NT = D / 8;
+    constexpr int CH = D >= 64 ? 16 : 8;  // bytes of K that a lane reads at once; columns of O it keeps: D / 4
+    constexpr int KY = D / (4 * CH);      // such reads of a row
+    constexpr int VB = D / 8;             // bytes of V that a lane reads of a row
+    extern __shared__ uint8_t smem_raw[];
+    Smem<D, MT, SPLIT>& sm =
+        *reinterpret_cast<Smem<D, MT, SPLIT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const CachedArgs& a = p.a;
+    const CacheArgs& b = a.cache;
+
+    pdl_launch();
+    if (tid == 0) {
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(&sm.full[i], 33);  // the copy's issuer and every lane's scales
+            mbar_init(&sm.empty[i], WARPS);
+        }
+        fence_barrier_init();
+    }
+    __syncthreads();
+    pdl_wait();
+
+    const int capacity = static_cast<int>(min(static_cast<long>(b.max_pages) << p.page_shift, 0x7FFFFFC0L));
+    Line<MR> line{a, p.G, lane, capacity};
+    const bool any = line.start(blockIdx.x, gridDim.x);
+    if (tid == 0) p.joins[blockIdx.x].first_cta = -1;
+    if (!any) return;
+    Piece x;
+    int st = 0, turn = 0;  // ring
+
+    if (warp == WARPS) {
+        // ------------------------------------------------------------ copies
+        const int frag_shift = min(p.page_shift, 6);  // a tile is 64 >> frag_shift stretches of a page
+        const int frags = TK >> frag_shift, frag = 1 << frag_shift;
+        if (lane == 0 && b.c.n_pages > 0 && b.max_pages > 0) {
+            prefetch_tensormap(&p.tk);
+            prefetch_tensormap(&p.tv);
+        }
+        while (line.next(x)) {
+            const int s = x.s;
+            for (int i = x.t0; i < x.t1; ++i) {
+                const int pos = i * TK + lane * frag;
+                int page = -1;
+                if (lane < frags && pos < x.len) page = page_of(b, p.page_shift, s, pos);
+                const unsigned ok = __ballot_sync(0xffffffffu, page >= 0);
+                if (turn > 0 && !mbar_wait_warp(&sm.empty[st], (turn - 1) & 1, a.wait_ns)) {
+                    // Copies still landing complete before the shared memory is released.
+                    for (int f = 0; f < C::STAGES; ++f) {
+                        mbar_wait(&sm.full[st], (turn - 1) & 1, 10000000ull);
+                        if (++st == C::STAGES) st = 0, ++turn;
+                    }
+                    if (lane == 0) atomicOr(a.status, 1);
+                    return;
+                }
+                if (lane == 0) {
+                    uint32_t bits = 0;
+                    for (int f = 0; f < frags; ++f)
+                        if ((ok >> f) & 1) bits |= ((1u << (frag >> 4)) - 1u) << (f * (frag >> 4));
+                    sm.valid[st] = bits;
+                    mbar_arrive_expect_tx(&sm.full[st], __popc(ok) * 2 * frag * D);
+                }
+                __syncwarp();
+                const int in_page = pos & (b.c.page_size - 1);
+                if (page >= 0) {
+                    const int row = (x.hk << p.page_shift) + in_page;
+                    tma_load_3d(sm.k[st] + lane * frag * D, &p.tk, 0, row, page, &sm.full[st]);
+                    tma_load_3d(sm.v[st] + lane * frag * D, &p.tv, 0, row, page, &sm.full[st]);
+                }
+                // Scales: lanes 0-15 four of K each, lanes 16-31 of V.
+                const int c4 = (lane & 15) * 4;
+                const int page4 = __shfl_sync(0xffffffffu, page, c4 >> frag_shift);
+                if (page4 >= 0) {
+                    const long row = ((static_cast<long>(page4) * b.c.n_kv_head + x.hk) << p.page_shift) +
+                                     ((i * TK + c4) & (b.c.page_size - 1));
+                    if (lane < 16) cp_async16(&sm.ks[st][c4], b.c.k_scale + row, 16);
+                    else cp_async16(&sm.vs[st][c4], b.c.v_scale + row, 16);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[st]))
+                             : "memory");
+                if (++st == C::STAGES) st = 0, ++turn;
+            }
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- products
+    bool dead = false;
+    while (line.next(x)) {
+        const int rows = min(x.n * p.G - x.row0, MR);
+        const int base = max(__ldg(b.kv_len + x.s), 0) - x.n;  // the first new position
+        // q as operand A: k slots (2t, 2t+1) and (2t+8, 2t+9) of step (y, i) are the four columns from
+        // 4 CH y + CH t + 4 i on.
+        uint32_t qh[C::Q_SMEM ? 1 : KS][MT][4], ql[SPLIT && !C::Q_SMEM ? KS : 1][MT][4];
+        float f[MT][2];               // a row's factor of the scores
+        int token[MT][2];
+        unsigned long long bits[MT][2];
+        if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);  // the piece before is done with q
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float4 w[2][KS];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 16 * mt + 8 * u + g, row = x.row0 + r;
+                const bool in = r < rows;
+                token[mt][u] = in ? row / p.G : -1;
+                const int h = x.hk * p.G + row % p.G;
+                const long at = static_cast<long>(x.q0 + token[mt][u]) * a.ld_q + h * D;
+                bits[mt][u] = in && a.tree ? __ldg(a.tree + x.q0 + token[mt][u]) : 0;
+                float most = 0.f;
+                bool finite = true;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    w[u][k] = in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float m4 = fmaxf(fmaxf(fabsf(w[u][k].x), fabsf(w[u][k].y)), fmaxf(fabsf(w[u][k].z), fabsf(w[u][k].w)));
+                    most = fmaxf(most, m4);
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                finite = most < INFINITY;
+                // The row times 2^(13 - e), e the exponent of its largest element.
+                const int e = finite ? max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) : 13;
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
+                const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
+                f[mt][u] = down * (a.scale * kLog2e) * Code::VALUE;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    w[u][k] = make_float4(w[u][k].x * up, w[u][k].y * up, w[u][k].z * up, w[u][k].w * up);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float4 v = w[u][k];
+                    hi[u] = pack_f16(v.x, v.y);
+                    hi[2 + u] = pack_f16(v.z, v.w);
+                    if constexpr (SPLIT) {
+                        const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[u]));
+                        const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[2 + u]));
+                        lo[u] = pack_f16(v.x - h0.x, v.y - h0.y);
+                        lo[2 + u] = pack_f16(v.z - h1.x, v.w - h1.y);
+                    }
+                }
+                if constexpr (C::Q_SMEM) {
+                    if (warp == (mt * KS + k) % WARPS) {
+                        sm.q[(k * MT + mt) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if constexpr (SPLIT)
+                            sm.q[((KS + k) * MT + mt) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        qh[k][mt][i] = hi[i];
+                        if constexpr (SPLIT) ql[k][mt][i] = lo[i];
+                    }
+                }
+            }
+        }
+        if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);
+
+        float o[MT][NT][4], m[MT][2], l[MT][2];
+        float unit = 0.f, w_in = 0.f;  // a power of two, at least the largest value scale so far; 2^7 / unit
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[mt][j][i] = 0.f;
+        }
+
+        for (int i = x.t0; i < x.t1; ++i) {
+            // After a wait that ran out the warp goes on without waiting or computing, to the CTA's barriers and its end.
+            if (!dead && !mbar_wait_warp(&sm.full[st], turn & 1, a.wait_ns)) {
+                dead = true;
+                if (lane == 0) atomicOr(a.status, 1);
+            }
+            const int pos0 = i * TK + warp * 16;
+            if (!dead && ((sm.valid[st] >> warp) & 1) && pos0 < x.len) {
+                const uint8_t* kt = sm.k[st] + warp * 16 * D;
+                const uint8_t* vt = sm.v[st] + warp * 16 * D;
+                // ---- S = q . codes of K
+                float s[MT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
+                uint32_t kw[2][KS];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    const int r = 8 * nt + tau<D>(g);
+#pragma unroll
+                    for (int y = 0; y < KY; ++y) {
+                        if constexpr (CH == 16) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(r, 4 * y + t));
+                            kw[nt][4 * y] = w.x;
+                            kw[nt][4 * y + 1] = w.y;
+                            kw[nt][4 * y + 2] = w.z;
+                            kw[nt][4 * y + 3] = w.w;
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(kt + chunk_at<D>(r, t >> 1) + 8 * (t & 1));
+                            kw[nt][0] = w.x;
+                            kw[nt][1] = w.y;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t b0[2], b1[2];
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const uint32_t w = Code::prepare(kw[nt][k]);
+                        b0[nt] = Code::template pair<0, 1>(w);
+                        b1[nt] = Code::template pair<2, 3>(w);
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        uint32_t ah[4], al[4];
+                        if constexpr (C::Q_SMEM) {
+                            const uint4 w = sm.q[(k * MT + mt) * 32 + lane];
+                            ah[0] = w.x, ah[1] = w.y, ah[2] = w.z, ah[3] = w.w;
+                            if constexpr (SPLIT) {
+                                const uint4 u = sm.q[((KS + k) * MT + mt) * 32 + lane];
+                                al[0] = u.x, al[1] = u.y, al[2] = u.z, al[3] = u.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                ah[c] = qh[k][mt][c];
+                                if constexpr (SPLIT) al[c] = ql[k][mt][c];
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) {
+                            mma16816(s[mt][nt], ah, b0[nt], b1[nt]);
+                            if constexpr (SPLIT) mma16816(s[mt][nt], al, b0[nt], b1[nt]);
+                        }
+                    }
+                }
+                // ---- scores, masks, row maxima
+                float vs[2][2], most = 0.f;
+                bool seen_all = pos0 + 16 <= min(base, x.len);
+                int where[2][2];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int r = 8 * nt + tau<D>(2 * t + c);
+                        where[nt][c] = pos0 + r;
+                        const float k_s = sm.ks[st][warp * 16 + r];
+                        vs[nt][c] = where[nt][c] < x.len ? sm.vs[st][warp * 16 + r] : 0.f;
+                        most = fmaxf(most, vs[nt][c]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) s[mt][nt][2 * u + c] *= k_s * f[mt][u];
+                    }
+                if (!seen_all) {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int j = where[nt][c] - base;  // the place among the new tokens
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    bool see = where[nt][c] < x.len;
+                                    if (j >= 0)
+                                        see = see && (a.tree ? j < 64 && ((bits[mt][u] >> j) & 1) : j <= token[mt][u]);
+                                    if (!see) s[mt][nt][2 * u + c] = -INFINITY;
+                                }
+                        }
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                bool raise = most > unit;
+                float mx[MT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float y = fmaxf(fmaxf(s[mt][0][2 * u], s[mt][0][2 * u + 1]), fmaxf(s[mt][1][2 * u], s[mt][1][2 * u + 1]));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+                        mx[mt][u] = y;
+                        raise |= y > m[mt][u] + RAISE;  // from -inf: any score
+                    }
+                if (__any_sync(0xffffffffu, raise)) {
+                    // unit: the next power of two.
+                    const float to = most > unit ? __uint_as_float((__float_as_uint(most) + 0x7FFFFFu) & 0x7F800000u) : unit;
+                    const float turn_unit = to > 0.f ? unit / to : 1.f;
+                    unit = to;
+                    w_in = to > 0.f ? W_UP / to : 0.f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            float r = 1.f;
+                            if (mx[mt][u] > m[mt][u] + RAISE) {
+                                r = ex2(m[mt][u] - mx[mt][u]);
+                                m[mt][u] = mx[mt][u];
+                            }
+                            l[mt][u] *= r;
+                            r *= turn_unit;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                o[mt][j][2 * u] *= r;
+                                o[mt][j][2 * u + 1] *= r;
+                            }
+                        }
+                }
+                // ---- weights as operand A
+                uint32_t ph[MT][4], pl[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float ref = m[mt][u] == -INFINITY ? 0.f : m[mt][u];
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) {
+                            float w[2];
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const float e = ex2(s[mt][nt][2 * u + c] - ref);
+                                l[mt][u] += e;
+                                // An unseen position's scale may be anything.
+                                w[c] = e == 0.f ? 0.f : e * (vs[nt][c] * w_in);
+                            }
+                            const uint32_t hi = pack_f16(w[0], w[1]);
+                            ph[mt][2 * nt + u] = hi;
+                            if constexpr (SPLIT) {
+                                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                                pl[mt][2 * nt + u] = pack_f16(w[0] - h.x, w[1] - h.y);
+                            }
+                        }
+                    }
+                // ---- O += weights . codes of V
+                uint32_t vw[4][VB / 4];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int r = 8 * nt + tau<D>(2 * t + c);
+                        if constexpr (VB == 16) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(r, g));
+                            vw[2 * nt + c][0] = w.x, vw[2 * nt + c][1] = w.y, vw[2 * nt + c][2] = w.z, vw[2 * nt + c][3] = w.w;
+                        } else if constexpr (VB == 8) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(r, g >> 1) + 8 * (g & 1));
+                            vw[2 * nt + c][0] = w.x, vw[2 * nt + c][1] = w.y;
+                        } else {
+                            vw[2 * nt + c][0] = *reinterpret_cast<const uint32_t*>(vt + chunk_at<D>(r, g >> 2) + 4 * (g & 3));
+                        }
+                    }
+#pragma unroll
+                for (int q = 0; q < VB / 4; ++q) {
+                    uint32_t z[2][2];  // two positions' bytes side by side: columns 4q, 4q+1 and 4q+2, 4q+3
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const uint32_t w0 = Code::prepare(vw[2 * nt][q]), w1 = Code::prepare(vw[2 * nt + 1][q]);
+                        z[nt][0] = prmt(w0, w1, 0x5140u);
+                        z[nt][1] = prmt(w0, w1, 0x7362u);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t b0 = c & 1 ? Code::template pair<2, 3>(z[0][c >> 1]) : Code::template pair<0, 1>(z[0][c >> 1]);
+                        const uint32_t b1 = c & 1 ? Code::template pair<2, 3>(z[1][c >> 1]) : Code::template pair<0, 1>(z[1][c >> 1]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816(o[mt][4 * q + c], ph[mt], b0, b1);
+                            if constexpr (SPLIT) mma16816(o[mt][4 * q + c], pl[mt], b0, b1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
+            if (++st == C::STAGES) st = 0, ++turn;
+        }
+
+        // ---- the four warps' parts into one: each scaled to the common maximum, then added in order
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 1);
+                l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 2);
+                if (t == 0) sm.ml[warp][16 * mt + 8 * u + g] = make_float2(m[mt][u], l[mt][u]);
+            }
+        named_sync(1, 32 * WARPS);
+        float mt_m[MT][2], mt_l[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float big = -INFINITY, sum = 0.f;
+                float2 e[WARPS];
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    e[w] = sm.ml[w][16 * mt + 8 * u + g];
+                    big = fmaxf(big, e[w].x);
+                }
+                const float ref = big == -INFINITY ? 0.f : big;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) sum += e[w].y * ex2(e[w].x - ref);
+                const float r = ex2(m[mt][u] - ref) * unit * (Code::VALUE / W_UP);
+                mt_m[mt][u] = big;
+                mt_l[mt][u] = sum;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    o[mt][j][2 * u] *= r;
+                    o[mt][j][2 * u + 1] *= r;
+                }
+            }
+        // Warps 2, 3 hand theirs to 0, 1, then 1 to 0.
+#pragma unroll
+        for (int half = 2; half >= 1; half >>= 1) {
+            if (warp >= half && warp < 2 * half) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        sm.o[warp - half][(mt * NT + j) * 32 + lane] =
+                            make_float4(o[mt][j][0], o[mt][j][1], o[mt][j][2], o[mt][j][3]);
+            }
+            named_sync(1, 32 * WARPS);
+            if (warp < half) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float4 y = sm.o[warp][(mt * NT + j) * 32 + lane];
+                        o[mt][j][0] += y.x;
+                        o[mt][j][1] += y.y;
+                        o[mt][j][2] += y.z;
+                        o[mt][j][3] += y.w;
+                    }
+            }
+            if (half == 2) named_sync(1, 32 * WARPS);
+        }
+        if (warp == 0) {
+            // A lane's columns of rows g and g+8: 2t * VB + j from c = 0, (2t + 1) * VB + j from c = 1.
+            const bool whole = x.t0 == 0 && x.t1 == x.tiles;
+            const int slot = 2 * blockIdx.x + (x.t0 == 0 ? 1 : 0);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = 16 * mt + 8 * u + g;
+                    if (r >= rows) continue;
+                    float y[2 * VB];
+                    const float inv = whole ? (mt_l[mt][u] == 0.f ? 0.f : 1.f / mt_l[mt][u]) : 1.f;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) y[c * VB + j] = o[mt][j][2 * u + c] * inv;
+                    if (whole) {
+                        const int h = x.hk * p.G + (x.row0 + r) % p.G;
+                        const long row = x.q0 + token[mt][u];
+                        store_out<2 * VB>(a, row * a.ld_o + h * D + 2 * VB * t, y);
+                        if (t == 0)
+                            a.lse[static_cast<long>(h) * b.N + row] =
+                                mt_l[mt][u] == 0.f ? -INFINITY : (mt_m[mt][u] + log2f(mt_l[mt][u])) * kLn2;
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + 2 * VB * t);
+#pragma unroll
+                        for (int q = 0; q < VB / 2; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+                        if (t == 0) p.part_ml[static_cast<long>(slot) * MR + r] = make_float2(mt_m[mt][u], mt_l[mt][u]);
+                    }
+                }
+            if (lane == 0 && x.t0 > 0 && x.t1 == x.tiles)
+                p.joins[blockIdx.x] = Join{line.owner(x.start), x.row0, rows, x.q0, x.hk};
+        }
+    }
+}
+
+// Adds the parts of the items that CTAs cut: block (c, y) the rows 4y .. 4y+3,
+// one warp each, of the item that CTA c ended.  The parts lie in the CTAs from
+// the join's first to c, one each, and are added in that order.
+template <int D, int MR>
+__global__ void __launch_bounds__(128) cached_join(const __grid_constant__ Params p) {
+    pdl_enter();
+    const CachedArgs& a = p.a;
+    const int c = blockIdx.x;
+    const Join j = p.joins[c];
+    const int r = 4 * blockIdx.y + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (j.first_cta < 0 || r >= j.rows) return;
+    constexpr int E = D / 32;
+    float acc[E], big = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int q0 = j.first_cta; q0 <= c; q0 += 32) {
+        // 32 parts at a time: a lane holds one's maximum and sum.
+        const int q = q0 + lane;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (q <= c) ml = p.part_ml[(2L * q + (q == j.first_cta ? 1 : 0)) * MR + r];
+        float top = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(top, big);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float keep = ex2(big - ref), w = ex2(ml.x - ref);
+        big = top;
+        float sum = ml.y * w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = fmaf(l, keep, sum);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= keep;
+        const int n = min(32, c + 1 - q0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* src = p.part_o + ((2L * (q0 + i) + (q0 + i == j.first_cta ? 1 : 0)) * MR + r) * D + lane * E;
+            float v[E];
+            if constexpr (E == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src);
+                v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+            } else if constexpr (E == 2) {
+                const float2 y = *reinterpret_cast<const float2*>(src);
+                v[0] = y.x, v[1] = y.y;
+            } else {
+                v[0] = *src;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(wi, v[e], acc[e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int row = j.row0 + r, h = j.hk * p.G + row % p.G;
+    const long at = j.q0 + row / p.G;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float y = acc[e] * inv;
+        const long i = at * a.ld_o + h * D + lane * E + e;
+        if (a.dtype == KATTN_F32) static_cast<float*>(a.o)[i] = y;
+        else if (a.dtype == KATTN_BF16) static_cast<__nv_bfloat16*>(a.o)[i] = __float2bfloat16_rn(y);
+        else static_cast<__half*>(a.o)[i] = __float2half_rn(y);
+    }
+    if (lane == 0) a.lse[static_cast<long>(h) * a.cache.N + at] = l == 0.f ? -INFINITY : (big + log2f(l)) * kLn2;
+}
+
+template <int D, int FORMAT, int MT, bool SPLIT>
+cudaError_t launch(Params& p, int ctas, bool join, cudaStream_t stream, int* launches) {
+    constexpr size_t smem = sizeof(Smem<D, MT, SPLIT>) + 1024;
+    static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs to an SM");
+    auto kernel = cached_fwd<D, FORMAT, MT, SPLIT>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> attr_done{0};  // one bit per device
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_done.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        attr_done.fetch_or(bit);
+    }
+    e = launch_pdl(kernel, dim3(ctas), dim3(N_THREADS), smem, stream, p);
+    if (e != cudaSuccess) return e;
+    ++*launches;
+    if (!join) return cudaSuccess;
+    e = launch_pdl(cached_join<D, 16 * MT>, dim3(ctas, 4 * MT), dim3(128), 0, stream, p);
+    if (e == cudaSuccess) ++*launches;
+    return e;
 }
 
 }  // namespace
 
 ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches) {
-    (void)pool;
+    const CacheArgs& b = a.cache;
+    const int D = b.c.d;
+    Params p{};
+    p.a = a;
+    p.page_shift = page_shift_of(b.c.page_size);
+    p.G = a.H / b.c.n_kv_head;
+    // Row tiles of 32 where the batch has more than 16 rows to a key head on average: they read the cache
+    // half as often; smaller ones leave more registers and half the idle rows.
+    const int MT = static_cast<long>(b.N) * p.G > 16L * b.S ? 2 : 1;
+    const int MR = 16 * MT, ctas = 2 * num_sms;
+    const bool join = (static_cast<long>(b.max_pages) << p.page_shift) > TK;  // else no item has two tiles
     ProjStatus st;
+    const size_t o_bytes = sizeof(float) * 2 * ctas * MR * D, ml_bytes = sizeof(float2) * 2 * ctas * MR;
+    char* ws = nullptr;
+    st.what = "cached forward workspace";
+    st.cuda = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), o_bytes + ml_bytes + sizeof(Join) * ctas, pool, s);
+    if (!st.ok()) return st;
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + o_bytes);
+    p.joins = reinterpret_cast<Join*>(ws + o_bytes + ml_bytes);
     st.what = "cached forward launch";
-    const long units = static_cast<long>(a.cache.N) * a.H;
-    const dim3 grid(static_cast<unsigned>(units / 4 + 1 < 16L * num_sms ? units / 4 + 1 : 16L * num_sms));
-    auto pick = [&](auto f32, auto bf16, auto f16) {
-        auto k = a.dtype == KATTN_F32 ? f32 : a.dtype == KATTN_BF16 ? bf16 : f16;
-        return launch_pdl(k, grid, dim3(128), 0, s, a, page_shift_of(a.cache.c.page_size));
-    };
-    auto size = [&](auto format) {
-        constexpr int F = decltype(format)::value;
-        const int d = a.cache.c.d;
-        return d == 32   ? pick(cached_rows<float, 32, F>, cached_rows<__nv_bfloat16, 32, F>, cached_rows<__half, 32, F>)
-               : d == 64 ? pick(cached_rows<float, 64, F>, cached_rows<__nv_bfloat16, 64, F>, cached_rows<__half, 64, F>)
-                         : pick(cached_rows<float, 128, F>, cached_rows<__nv_bfloat16, 128, F>, cached_rows<__half, 128, F>);
-    };
-    st.cuda = a.cache.c.format == KATTN_CACHE_INT8 ? size(std::integral_constant<int, KATTN_CACHE_INT8>{})
-                                                   : size(std::integral_constant<int, KATTN_CACHE_E4M3>{});
-    if (st.ok()) ++*launches;
+    if (b.c.n_pages > 0 && b.max_pages > 0) {
+        const CUtensorMapSwizzle sw = D == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                      : D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+        const int rows = std::min(b.c.page_size, TK);
+        if (!encode_pages(&p.tk, b.c.k, b.c.n_pages, b.c.n_kv_head * b.c.page_size, D, rows, sw) ||
+            !encode_pages(&p.tv, b.c.v, b.c.n_pages, b.c.n_kv_head * b.c.page_size, D, rows, sw))
+            st.cuda = cudaErrorInvalidValue;
+    }
+    if (st.ok()) {
+        auto pick = [&](auto d, auto fmt, auto mt, auto split) {
+            return launch<decltype(d)::value, decltype(fmt)::value, decltype(mt)::value, decltype(split)::value>(
+                p, ctas, join, s, launches);
+        };
+        auto by_split = [&](auto d, auto fmt, auto mt) {
+            return a.dtype == KATTN_F32 ? pick(d, fmt, mt, std::true_type{}) : pick(d, fmt, mt, std::false_type{});
+        };
+        auto by_mt = [&](auto d, auto fmt) {
+            return MT == 1 ? by_split(d, fmt, std::integral_constant<int, 1>{})
+                           : by_split(d, fmt, std::integral_constant<int, 2>{});
+        };
+        auto by_format = [&](auto d) {
+            return b.c.format == KATTN_CACHE_INT8 ? by_mt(d, std::integral_constant<int, KATTN_CACHE_INT8>{})
+                                                  : by_mt(d, std::integral_constant<int, KATTN_CACHE_E4M3>{});
+        };
+        st.cuda = D == 32   ? by_format(std::integral_constant<int, 32>{})
+                  : D == 64 ? by_format(std::integral_constant<int, 64>{})
+                            : by_format(std::integral_constant<int, 128>{});
+    }
+    const cudaError_t freed = cudaFreeAsync(ws, s);
+    if (st.ok()) st.cuda = freed;
     return st;
 }
 

@@ -193,7 +193,7 @@ int kattn_fwd_cached(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, con
     DeviceScope scope(ctx->device);
     if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
     const kattn::CachedArgs a{{*cache, cu, kv_len, table, ld_table, max_pages, S, N}, dtype, q, ld_q, o, ld_o, lse,
-                              tree, H, scale};
+                              tree, H, scale, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed)};
     int launches = 0;
     const kattn::ProjStatus st =
         kattn::cached_forward(a, ctx->num_sms, ctx->pool, static_cast<cudaStream_t>(stream), &launches);

@@ -26,4 +26,9 @@ bool encode_2d(CUtensorMap* map, const float* base, long cols, long rows, long l
 bool encode_2d_bf16(CUtensorMap* map, const uint16_t* base, long cols, long rows, long ld, int box_cols, int box_rows,
                     CUtensorMapSwizzle swizzle);
 
+// Pages of 8-bit rows, [n_pages][rows][cols] contiguous bytes, as a 3-D tensor
+// {cols, rows, n_pages}, boxes of whole rows, box_rows of one page.
+bool encode_pages(CUtensorMap* map, const void* base, int n_pages, int rows, int cols, int box_rows,
+                  CUtensorMapSwizzle swizzle);
+
 }  // namespace kattn
