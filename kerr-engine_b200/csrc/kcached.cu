@@ -11,9 +11,11 @@
 // MMA operands with few instructions.
 //
 // Rows.  The G query heads of a key head share its positions: a sequence's n
-// tokens are n * G rows, in row tiles of 16 * MT, the m of mma.m16n8k16.
+// tokens are n * G rows, in row tiles of 8 * NB.  Positions are the m of
+// mma.m16n8k16 and rows its n, so that a tile of few rows wastes few products:
+// S^T = K q^T, then O^T = V^T P^T with P^T turned in registers.
 //
-// Split.  The (sequence, key head, row tile) items and their tiles of 64 positions
+// Split.  The (sequence, key head, row tile) items and their tiles of positions
 // are one line of work, cut into as many equal parts as there are CTAs
 // (two to an SM), whatever the lengths; an item cut by a border leaves parts
 // (row maxima, sums, O) in a workspace, which cached_join adds in order.
@@ -24,11 +26,10 @@
 // of it; f32 as a hi / lo pair), the weights p_j vs_j to f16 after a power of two
 // per warp (f32: as a pair).  The scale ks_j multiplies the score.
 //
-// A warp takes 16 of a tile's 64 positions.  Its lanes read whole 16-byte chunks
-// of codes: the order of d in the first product is free (q is permuted
-// alike), and in the second a lane's chunk spreads over 16 of the n8 tiles, which
-// leaves it 32 neighbouring columns of O.  tau() orders a tile's positions so that
-// both reads meet no bank twice under the copy's swizzle.
+// Lanes read whole 16-byte chunks of codes: the order of d in the first product
+// is free (q is permuted alike), and in the second a lane's chunk spreads over
+// the m of 8 MMAs, which leaves it 16 neighbouring columns of O.  tau() orders eight
+// positions so that both reads meet no bank twice under the copy's swizzle.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -46,10 +47,13 @@ namespace {
 using namespace serve;
 using namespace sm100;
 
-constexpr int TK = 64;     // positions of a tile
-constexpr int WARPS = 4;   // computing warps, 16 positions of a tile each
-constexpr int N_THREADS = 32 * (WARPS + 1);
+constexpr int TK = 128;              // positions of a tile
+constexpr int WARPS = 4;             // computing warps, 32 positions of a tile each
+// A warpgroup computes and one of another issues the copies (its other warps only lend their registers): two
+// such CTAs to an SM.
+constexpr int N_THREADS = 256, R_COMPUTE = 208, R_COPY = 48;
 constexpr float RAISE = 8.f;         // a row's reference is raised when its maximum passes it by 2^8
+constexpr int EXTRA = 2;             // what an item's rows, joins and stores cost, in tiles
 constexpr float W_UP = 128.f;        // weights are held times 2^7: at most 2^15 with RAISE, far from f16's subnormals
 
 // A part's place in the line of work, and what joins it.
@@ -68,26 +72,27 @@ struct Params {
     Join* joins;     // [CTAs]
 };
 
-template <int D, int MT, bool SPLIT>
+template <int D, int NB, bool SPLIT>
 struct Cfg {
-    static constexpr int MR = 16 * MT;
-    static constexpr int KS = D / 16;                      // k steps of the first product
-    static constexpr bool Q_SMEM = MT > 1;                 // q in shared memory (registers are O's)
-    static constexpr int Q_WORDS = Q_SMEM ? KS * MT * (SPLIT ? 2 : 1) * 32 : 1;
-    static constexpr int STAGES = MT > 1 && D == 128 ? 3 : 4;
+    static constexpr int MR = 8 * NB;
+    static constexpr int KS = D / 16;                          // k steps of the first product
+    static constexpr int GR = NB > 2 ? 1 : 2;                  // groups of 16 positions a warp takes at once
+    static constexpr bool Q_SMEM = NB * D * (SPLIT ? 2 : 1) > 256;  // q in shared memory rather than registers
+    static constexpr int Q_WORDS = Q_SMEM ? KS * NB * (SPLIT ? 2 : 1) * 32 : 1;
+    static constexpr int FIT = (106 * 1024 - WARPS / 2 * MR * D * 4 - 8 * Q_WORDS) / (2 * TK * (D + 4));
+    static constexpr int STAGES = FIT < 6 ? FIT : 6;
 };
 
-template <int D, int MT, bool SPLIT>
+template <int D, int NB, bool SPLIT>
 struct Smem {
-    using C = Cfg<D, MT, SPLIT>;
+    using C = Cfg<D, NB, SPLIT>;
     alignas(1024) uint8_t k[C::STAGES][TK * D];
     alignas(1024) uint8_t v[C::STAGES][TK * D];
     alignas(16) float ks[C::STAGES][TK];
     alignas(16) float vs[C::STAGES][TK];
-    alignas(16) uint4 q[C::Q_WORDS];
-    alignas(16) float4 o[2][C::MR * D / 4];  // exchange of two warps' O
+    alignas(16) uint2 q[C::Q_WORDS];
+    alignas(16) float4 o[WARPS / 2][C::MR * D / 4];  // O of half the warps, handed to the other
     float2 ml[WARPS][C::MR];
-    float unit[WARPS];
     uint32_t valid[C::STAGES];  // a bit for each 16 positions: they exist
     uint64_t full[C::STAGES], empty[C::STAGES];
 };
@@ -114,6 +119,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The 8x8 matrix of 16-bit elements whose row lane / 4 has its columns 2 (lane % 4)
+// and the next in x, transposed.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -150,9 +163,10 @@ struct Piece {
     int s, q0, n, len;   // sequence, its first row, rows and length
     int hk, row0;        // key head, first row of the row tile
     int t0, t1, tiles;   // its tiles t0 .. t1-1 of the item's
-    long start;          // the item's first tile in the line
+    long first;          // the place of its first tile in the line
 };
 
+// An item counts EXTRA tiles before its own.
 template <int MR>
 struct Line {
     const CachedArgs& a;
@@ -169,7 +183,10 @@ struct Line {
         len = min(max(__ldg(a.cache.kv_len + i), 0), capacity);
         row_tiles = (n * G + MR - 1) / MR;
         tiles = max(1, (len + TK - 1) / TK);
-        return static_cast<long>(row_tiles) * a.cache.c.n_kv_head * tiles;
+        return sequence();
+    }
+    __device__ __forceinline__ long sequence() const {
+        return static_cast<long>(row_tiles) * a.cache.c.n_kv_head * (tiles + EXTRA);
     }
     // Finds the CTA's part; whole warps.
     __device__ __forceinline__ bool start(int cta, int grid) {
@@ -206,25 +223,28 @@ struct Line {
     }
     // The next piece of the CTA's part; false: none is left.
     __device__ __forceinline__ bool next(Piece& p) {
-        if (at >= end) return false;
-        long mine = static_cast<long>(row_tiles) * a.cache.c.n_kv_head * tiles;
-        while (at >= base + mine) {
-            base += mine;
-            mine = load(++s);
+        while (at < end) {
+            long mine = sequence();
+            while (at >= base + mine) {
+                base += mine;
+                mine = load(++s);
+            }
+            const int item = static_cast<int>((at - base) / (tiles + EXTRA));
+            p.s = s;
+            p.q0 = q0;
+            p.n = n;
+            p.len = len;
+            p.hk = item / row_tiles;
+            p.row0 = (item % row_tiles) * MR;
+            p.tiles = tiles;
+            p.first = base + static_cast<long>(item) * (tiles + EXTRA) + EXTRA;
+            p.t0 = static_cast<int>(max(at - p.first, 0L));
+            p.t1 = static_cast<int>(min(static_cast<long>(tiles), end - p.first));
+            at = p.first + p.t1;
+            if (p.t1 > p.t0) return true;
+            at = end;  // the border lies before the item's first tile
         }
-        const int item = static_cast<int>((at - base) / tiles);
-        p.s = s;
-        p.q0 = q0;
-        p.n = n;
-        p.len = len;
-        p.hk = item / row_tiles;
-        p.row0 = (item % row_tiles) * MR;
-        p.tiles = tiles;
-        p.start = base + static_cast<long>(item) * tiles;
-        p.t0 = static_cast<int>(at - p.start);
-        p.t1 = static_cast<int>(min(static_cast<long>(tiles), end - p.start));
-        at = p.start + p.t1;
-        return true;
+        return false;
     }
     // The CTA that holds the line's tile g.
     __device__ __forceinline__ int owner(long g) const { return static_cast<int>(((g + 1) * ctas + total - 1) / total) - 1; }
@@ -260,17 +280,18 @@ __device__ __forceinline__ void store_out(const CachedArgs& a, long i, const flo
 }
 
 // ---------------------------------------------------------------- kernel
-template <int D, int FORMAT, int MT, bool SPLIT>
+template <int D, int FORMAT, int NB, bool SPLIT>
 __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant__ Params p) {
-    using C = Cfg<D, MT, SPLIT>;
+    using C = Cfg<D, NB, SPLIT>;
     using Code = Codes<FORMAT>;
-    constexpr int MR = C::MR, KS = C::KS, NT = D / 8;
-    constexpr int CH = D >= 64 ? 16 : 8;  // bytes of K that a lane reads at once; columns of O it keeps: D / 4
+    constexpr int MR = C::MR, KS = C::KS, GR = C::GR;
+    constexpr int CH = D >= 64 ? 16 : 8;  // bytes of K that a lane reads at once
     constexpr int KY = D / (4 * CH);      // such reads of a row
-    constexpr int VB = D / 8;             // bytes of V that a lane reads of a row
+    constexpr int VB = D / 8;             // bytes of V that a lane reads of a row, columns of O that it keeps
+    constexpr int NJ = VB / 2;            // MMAs of the second product, two of those columns each
     extern __shared__ uint8_t smem_raw[];
-    Smem<D, MT, SPLIT>& sm =
-        *reinterpret_cast<Smem<D, MT, SPLIT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Smem<D, NB, SPLIT>& sm =
+        *reinterpret_cast<Smem<D, NB, SPLIT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const CachedArgs& a = p.a;
     const CacheArgs& b = a.cache;
@@ -294,9 +315,11 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     Piece x;
     int st = 0, turn = 0;  // ring
 
-    if (warp == WARPS) {
+    if (warp >= WARPS) {
         // ------------------------------------------------------------ copies
-        const int frag_shift = min(p.page_shift, 6);  // a tile is 64 >> frag_shift stretches of a page
+        regs_dec<R_COPY>();
+        if (warp > WARPS) return;
+        const int frag_shift = min(p.page_shift, 7);  // a tile is TK >> frag_shift stretches of a page
         const int frags = TK >> frag_shift, frag = 1 << frag_shift;
         if (lane == 0 && b.c.n_pages > 0 && b.max_pages > 0) {
             prefetch_tensormap(&p.tk);
@@ -332,14 +355,14 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                     tma_load_3d(sm.k[st] + lane * frag * D, &p.tk, 0, row, page, &sm.full[st]);
                     tma_load_3d(sm.v[st] + lane * frag * D, &p.tv, 0, row, page, &sm.full[st]);
                 }
-                // Scales: lanes 0-15 four of K each, lanes 16-31 of V.
-                const int c4 = (lane & 15) * 4;
+                // Scales, four of each a lane.
+                const int c4 = lane * 4;
                 const int page4 = __shfl_sync(0xffffffffu, page, c4 >> frag_shift);
                 if (page4 >= 0) {
                     const long row = ((static_cast<long>(page4) * b.c.n_kv_head + x.hk) << p.page_shift) +
                                      ((i * TK + c4) & (b.c.page_size - 1));
-                    if (lane < 16) cp_async16(&sm.ks[st][c4], b.c.k_scale + row, 16);
-                    else cp_async16(&sm.vs[st][c4], b.c.v_scale + row, 16);
+                    cp_async16(&sm.ks[st][c4], b.c.k_scale + row, 16);
+                    cp_async16(&sm.vs[st][c4], b.c.v_scale + row, 16);
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[st]))
                              : "memory");
@@ -350,91 +373,72 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     }
 
     // ---------------------------------------------------------------- products
+    regs_inc<R_COMPUTE>();
+    // This lane's rows are 8 nb + 2t + c; the statistics of a row are the same in its eight lanes.
     bool dead = false;
     while (line.next(x)) {
         const int rows = min(x.n * p.G - x.row0, MR);
         const int base = max(__ldg(b.kv_len + x.s), 0) - x.n;  // the first new position
-        // q as operand A: k slots (2t, 2t+1) and (2t+8, 2t+9) of step (y, i) are the four columns from
-        // 4 CH y + CH t + 4 i on.
-        uint32_t qh[C::Q_SMEM ? 1 : KS][MT][4], ql[SPLIT && !C::Q_SMEM ? KS : 1][MT][4];
-        float f[MT][2];               // a row's factor of the scores
-        int token[MT][2];
-        unsigned long long bits[MT][2];
+        // q as operand B, row 8 nb + g: k slots (2t, 2t+1) and (2t+8, 2t+9) of step k are four neighbouring columns.
+        uint2 qh[C::Q_SMEM ? 1 : KS][NB], ql[SPLIT && !C::Q_SMEM ? KS : 1][NB];
+        float f[NB][2];  // factors of the rows' scores
         if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);  // the piece before is done with q
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float4 w[2][KS];
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g, row = x.row0 + r;
+            const bool in = r < rows;
+            const long at = static_cast<long>(x.q0 + row / p.G) * a.ld_q + (x.hk * p.G + row % p.G) * D;
+            float4 w[KS];
+            float most = 0.f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r = 16 * mt + 8 * u + g, row = x.row0 + r;
-                const bool in = r < rows;
-                token[mt][u] = in ? row / p.G : -1;
-                const int h = x.hk * p.G + row % p.G;
-                const long at = static_cast<long>(x.q0 + token[mt][u]) * a.ld_q + h * D;
-                bits[mt][u] = in && a.tree ? __ldg(a.tree + x.q0 + token[mt][u]) : 0;
-                float most = 0.f;
-                bool finite = true;
+            for (int k = 0; k < KS; ++k) {
+                w[k] = in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(w[k].x), fabsf(w[k].y)), fmaxf(fabsf(w[k].z), fabsf(w[k].w))));
+            }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            // The row times 2^(13 - e), e the exponent of its largest element.
+            const int e = most < INFINITY ? max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) : 13;
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    w[u][k] = in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-                    const float m4 = fmaxf(fmaxf(fabsf(w[u][k].x), fabsf(w[u][k].y)), fmaxf(fabsf(w[u][k].z), fabsf(w[u][k].w)));
-                    most = fmaxf(most, m4);
-                }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                finite = most < INFINITY;
-                // The row times 2^(13 - e), e the exponent of its largest element.
-                const int e = finite ? max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) : 13;
-                const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
-                const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
-                f[mt][u] = down * (a.scale * kLog2e) * Code::VALUE;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-                    w[u][k] = make_float4(w[u][k].x * up, w[u][k].y * up, w[u][k].z * up, w[u][k].w * up);
+            for (int c = 0; c < 2; ++c) {
+                f[nb][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * (a.scale * kLog2e) * Code::VALUE;
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float4 v = w[u][k];
-                    hi[u] = pack_f16(v.x, v.y);
-                    hi[2 + u] = pack_f16(v.z, v.w);
-                    if constexpr (SPLIT) {
-                        const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[u]));
-                        const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[2 + u]));
-                        lo[u] = pack_f16(v.x - h0.x, v.y - h0.y);
-                        lo[2 + u] = pack_f16(v.z - h1.x, v.w - h1.y);
-                    }
+                const float4 v = make_float4(w[k].x * up, w[k].y * up, w[k].z * up, w[k].w * up);
+                const uint2 hi = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+                uint2 lo = make_uint2(0, 0);
+                if constexpr (SPLIT) {
+                    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                    lo = make_uint2(pack_f16(v.x - h0.x, v.y - h0.y), pack_f16(v.z - h1.x, v.w - h1.y));
                 }
                 if constexpr (C::Q_SMEM) {
-                    if (warp == (mt * KS + k) % WARPS) {
-                        sm.q[(k * MT + mt) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if constexpr (SPLIT)
-                            sm.q[((KS + k) * MT + mt) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (warp == nb % WARPS) {
+                        sm.q[(k * NB + nb) * 32 + lane] = hi;
+                        if constexpr (SPLIT) sm.q[((KS + k) * NB + nb) * 32 + lane] = lo;
                     }
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        qh[k][mt][i] = hi[i];
-                        if constexpr (SPLIT) ql[k][mt][i] = lo[i];
-                    }
+                    qh[k][nb] = hi;
+                    if constexpr (SPLIT) ql[k][nb] = lo;
                 }
             }
         }
         if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);
 
-        float o[MT][NT][4], m[MT][2], l[MT][2];
+        float o[NB][NJ][4], m[NB][2], l[NB][2];
         float unit = 0.f, w_in = 0.f;  // a power of two, at least the largest value scale so far; 2^7 / unit
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[mt][j][i] = 0.f;
+                for (int i = 0; i < 4; ++i) o[nb][j][i] = 0.f;
         }
 
         for (int i = x.t0; i < x.t1; ++i) {
@@ -443,202 +447,196 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 dead = true;
                 if (lane == 0) atomicOr(a.status, 1);
             }
-            const int pos0 = i * TK + warp * 16;
-            if (!dead && ((sm.valid[st] >> warp) & 1) && pos0 < x.len) {
-                const uint8_t* kt = sm.k[st] + warp * 16 * D;
-                const uint8_t* vt = sm.v[st] + warp * 16 * D;
-                // ---- S = q . codes of K
-                float s[MT][2][4];
+#pragma unroll 1
+            for (int step = 0; step < 2 / GR; ++step) {
+                const int group = warp * 2 + step * GR;  // of 16 positions
+                const int pos0 = i * TK + group * 16;
+                const uint32_t here = (sm.valid[st] >> group) & ((1u << GR) - 1u);
+                if (dead || here == 0 || pos0 >= x.len) continue;
+                const uint8_t* kt = sm.k[st] + group * 16 * D;
+                const uint8_t* vt = sm.v[st] + group * 16 * D;
+                // ---- S^T = codes of K . q
+                float s[GR][NB][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int gr = 0; gr < GR; ++gr) {
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
-                uint32_t kw[2][KS];
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const int r = 8 * nt + tau<D>(g);
-#pragma unroll
-                    for (int y = 0; y < KY; ++y) {
-                        if constexpr (CH == 16) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(r, 4 * y + t));
-                            kw[nt][4 * y] = w.x;
-                            kw[nt][4 * y + 1] = w.y;
-                            kw[nt][4 * y + 2] = w.z;
-                            kw[nt][4 * y + 3] = w.w;
-                        } else {
-                            const uint2 w = *reinterpret_cast<const uint2*>(kt + chunk_at<D>(r, t >> 1) + 8 * (t & 1));
-                            kw[nt][0] = w.x;
-                            kw[nt][1] = w.y;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    uint32_t b0[2], b1[2];
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const uint32_t w = Code::prepare(kw[nt][k]);
-                        b0[nt] = Code::template pair<0, 1>(w);
-                        b1[nt] = Code::template pair<2, 3>(w);
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t ah[4], al[4];
-                        if constexpr (C::Q_SMEM) {
-                            const uint4 w = sm.q[(k * MT + mt) * 32 + lane];
-                            ah[0] = w.x, ah[1] = w.y, ah[2] = w.z, ah[3] = w.w;
-                            if constexpr (SPLIT) {
-                                const uint4 u = sm.q[((KS + k) * MT + mt) * 32 + lane];
-                                al[0] = u.x, al[1] = u.y, al[2] = u.z, al[3] = u.w;
-                            }
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                ah[c] = qh[k][mt][c];
-                                if constexpr (SPLIT) al[c] = ql[k][mt][c];
-                            }
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) {
-                            mma16816(s[mt][nt], ah, b0[nt], b1[nt]);
-                            if constexpr (SPLIT) mma16816(s[mt][nt], al, b0[nt], b1[nt]);
-                        }
-                    }
-                }
-                // ---- scores, masks, row maxima
-                float vs[2][2], most = 0.f;
-                bool seen_all = pos0 + 16 <= min(base, x.len);
-                int where[2][2];
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int r = 8 * nt + tau<D>(2 * t + c);
-                        where[nt][c] = pos0 + r;
-                        const float k_s = sm.ks[st][warp * 16 + r];
-                        vs[nt][c] = where[nt][c] < x.len ? sm.vs[st][warp * 16 + r] : 0.f;
-                        most = fmaxf(most, vs[nt][c]);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) s[mt][nt][2 * u + c] *= k_s * f[mt][u];
-                    }
-                if (!seen_all) {
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int j = where[nt][c] - base;  // the place among the new tokens
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                                for (int u = 0; u < 2; ++u) {
-                                    bool see = where[nt][c] < x.len;
-                                    if (j >= 0)
-                                        see = see && (a.tree ? j < 64 && ((bits[mt][u] >> j) & 1) : j <= token[mt][u]);
-                                    if (!see) s[mt][nt][2 * u + c] = -INFINITY;
-                                }
-                        }
-                }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                bool raise = most > unit;
-                float mx[MT][2];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                        for (int c = 0; c < 4; ++c) s[gr][nb][c] = 0.f;
+                    uint32_t kw[2][KS];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        float y = fmaxf(fmaxf(s[mt][0][2 * u], s[mt][0][2 * u + 1]), fmaxf(s[mt][1][2 * u], s[mt][1][2 * u + 1]));
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-                        mx[mt][u] = y;
-                        raise |= y > m[mt][u] + RAISE;  // from -inf: any score
+                        const int r = 16 * gr + 8 * u + tau<D>(g);
+#pragma unroll
+                        for (int y = 0; y < KY; ++y) {
+                            if constexpr (CH == 16) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(r, 4 * y + t));
+                                kw[u][4 * y] = w.x;
+                                kw[u][4 * y + 1] = w.y;
+                                kw[u][4 * y + 2] = w.z;
+                                kw[u][4 * y + 3] = w.w;
+                            } else {
+                                const uint2 w = *reinterpret_cast<const uint2*>(kt + chunk_at<D>(r, t >> 1) + 8 * (t & 1));
+                                kw[u][0] = w.x;
+                                kw[u][1] = w.y;
+                            }
+                        }
                     }
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const uint32_t w0 = Code::prepare(kw[0][k]), w1 = Code::prepare(kw[1][k]);
+                        const uint32_t ka[4] = {Code::template pair<0, 1>(w0), Code::template pair<0, 1>(w1),
+                                                Code::template pair<2, 3>(w0), Code::template pair<2, 3>(w1)};
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const uint2 h = C::Q_SMEM ? sm.q[(k * NB + nb) * 32 + lane] : qh[C::Q_SMEM ? 0 : k][nb];
+                            mma16816(s[gr][nb], ka, h.x, h.y);
+                            if constexpr (SPLIT) {
+                                const uint2 e = C::Q_SMEM ? sm.q[((KS + k) * NB + nb) * 32 + lane] : ql[C::Q_SMEM ? 0 : k][nb];
+                                mma16816(s[gr][nb], ka, e.x, e.y);
+                            }
+                        }
+                    }
+                }
+                // ---- scores and masks
+                const bool seen_all = pos0 + 16 * GR <= min(base, x.len) && here == (1u << GR) - 1u;
+                float vs[GR][2];
+                bool raise = false;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int r = 16 * gr + 8 * u + tau<D>(g);
+                        const float k_s = sm.ks[st][group * 16 + r];
+                        vs[gr][u] = sm.vs[st][group * 16 + r];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) s[gr][nb][2 * u + c] *= k_s * f[nb][c];
+                        if (!seen_all) {
+                            const int pos = pos0 + r, j = pos - base;  // j: the place among the new tokens
+                            const bool exists = pos < x.len && ((here >> gr) & 1);
+                            if (!exists) vs[gr][u] = 0.f;
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    const int mine = 8 * nb + 2 * t + c, token = (x.row0 + mine) / p.G;
+                                    bool see = exists && mine < rows;
+                                    if (see && j >= 0)
+                                        see = a.tree ? j < 64 && ((__ldg(a.tree + x.q0 + token) >> j) & 1) : j <= token;
+                                    if (!see) s[gr][nb][2 * u + c] = -INFINITY;
+                                }
+                        }
+                        raise |= vs[gr][u] > unit;
+                    }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float y = fmaxf(s[0][nb][c], s[0][nb][2 + c]);
+                        if constexpr (GR == 2) y = fmaxf(y, fmaxf(s[GR - 1][nb][c], s[GR - 1][nb][2 + c]));
+                        raise |= y > m[nb][c] + RAISE;  // from -inf: any score
+                    }
+                // The references rise seldom, so only then are the warp's maxima formed.
                 if (__any_sync(0xffffffffu, raise)) {
+                    float most = 0.f;
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr) most = fmaxf(most, fmaxf(vs[gr][0], vs[gr][1]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
                     // unit: the next power of two.
                     const float to = most > unit ? __uint_as_float((__float_as_uint(most) + 0x7FFFFFu) & 0x7F800000u) : unit;
                     const float turn_unit = to > 0.f ? unit / to : 1.f;
                     unit = to;
                     w_in = to > 0.f ? W_UP / to : 0.f;
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        for (int c = 0; c < 2; ++c) {
+                            float y = fmaxf(s[0][nb][c], s[0][nb][2 + c]);
+                            if constexpr (GR == 2) y = fmaxf(y, fmaxf(s[GR - 1][nb][c], s[GR - 1][nb][2 + c]));
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
                             float r = 1.f;
-                            if (mx[mt][u] > m[mt][u] + RAISE) {
-                                r = ex2(m[mt][u] - mx[mt][u]);
-                                m[mt][u] = mx[mt][u];
+                            if (y > m[nb][c] + RAISE) {
+                                r = ex2(m[nb][c] - y);
+                                m[nb][c] = y;
                             }
-                            l[mt][u] *= r;
+                            l[nb][c] *= r;
                             r *= turn_unit;
 #pragma unroll
-                            for (int j = 0; j < NT; ++j) {
-                                o[mt][j][2 * u] *= r;
-                                o[mt][j][2 * u + 1] *= r;
+                            for (int j = 0; j < NJ; ++j) {
+                                o[nb][j][c] *= r;
+                                o[nb][j][2 + c] *= r;
                             }
                         }
                 }
-                // ---- weights as operand A
-                uint32_t ph[MT][4], pl[MT][4];
+                // ---- weights as operand B
+                uint2 ph[GR][NB], pl[SPLIT ? GR : 1][NB];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float ref = m[mt][u] == -INFINITY ? 0.f : m[mt][u];
+                    for (int nb = 0; nb < NB; ++nb) {
+                        uint32_t h[2], e[2];
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) {
+                        for (int u = 0; u < 2; ++u) {
                             float w[2];
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                const float e = ex2(s[mt][nt][2 * u + c] - ref);
-                                l[mt][u] += e;
-                                // An unseen position's scale may be anything.
-                                w[c] = e == 0.f ? 0.f : e * (vs[nt][c] * w_in);
+                                const float ref = m[nb][c] == -INFINITY ? 0.f : m[nb][c];
+                                const float q = ex2(s[gr][nb][2 * u + c] - ref);
+                                l[nb][c] += q;
+                                w[c] = q * (vs[gr][u] * w_in);
+                                if (!seen_all && q == 0.f) w[c] = 0.f;  // an unseen position's scale may be a NaN
                             }
-                            const uint32_t hi = pack_f16(w[0], w[1]);
-                            ph[mt][2 * nt + u] = hi;
+                            h[u] = pack_f16(w[0], w[1]);
                             if constexpr (SPLIT) {
-                                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                                pl[mt][2 * nt + u] = pack_f16(w[0] - h.x, w[1] - h.y);
+                                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[u]));
+                                e[u] = pack_f16(w[0] - y.x, w[1] - y.y);
                             }
                         }
+                        ph[gr][nb] = make_uint2(turned(h[0]), turned(h[1]));
+                        if constexpr (SPLIT) pl[gr][nb] = make_uint2(turned(e[0]), turned(e[1]));
                     }
-                // ---- O += weights . codes of V
-                uint32_t vw[4][VB / 4];
+                // ---- O^T += codes of V^T . weights
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int gr = 0; gr < GR; ++gr) {
+                    uint32_t vw[4][VB / 4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int r = 8 * nt + tau<D>(2 * t + c);
-                        if constexpr (VB == 16) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(r, g));
-                            vw[2 * nt + c][0] = w.x, vw[2 * nt + c][1] = w.y, vw[2 * nt + c][2] = w.z, vw[2 * nt + c][3] = w.w;
-                        } else if constexpr (VB == 8) {
-                            const uint2 w = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(r, g >> 1) + 8 * (g & 1));
-                            vw[2 * nt + c][0] = w.x, vw[2 * nt + c][1] = w.y;
-                        } else {
-                            vw[2 * nt + c][0] = *reinterpret_cast<const uint32_t*>(vt + chunk_at<D>(r, g >> 2) + 4 * (g & 3));
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int r = 16 * gr + 8 * u + tau<D>(2 * t + c);
+                            uint32_t(&to)[VB / 4] = vw[2 * u + c];
+                            if constexpr (VB == 16) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(r, g));
+                                to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+                            } else if constexpr (VB == 8) {
+                                const uint2 w = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(r, g >> 1) + 8 * (g & 1));
+                                to[0] = w.x, to[1] = w.y;
+                            } else {
+                                to[0] = *reinterpret_cast<const uint32_t*>(vt + chunk_at<D>(r, g >> 2) + 4 * (g & 3));
+                            }
                         }
-                    }
 #pragma unroll
-                for (int q = 0; q < VB / 4; ++q) {
-                    uint32_t z[2][2];  // two positions' bytes side by side: columns 4q, 4q+1 and 4q+2, 4q+3
+                    for (int q = 0; q < VB / 4; ++q) {
+                        uint32_t z[2][2];  // two positions' bytes side by side: columns 4q, 4q+1 and 4q+2, 4q+3
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const uint32_t w0 = Code::prepare(vw[2 * nt][q]), w1 = Code::prepare(vw[2 * nt + 1][q]);
-                        z[nt][0] = prmt(w0, w1, 0x5140u);
-                        z[nt][1] = prmt(w0, w1, 0x7362u);
-                    }
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t w0 = Code::prepare(vw[2 * u][q]), w1 = Code::prepare(vw[2 * u + 1][q]);
+                            z[u][0] = prmt(w0, w1, 0x5140u);
+                            z[u][1] = prmt(w0, w1, 0x7362u);
+                        }
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t b0 = c & 1 ? Code::template pair<2, 3>(z[0][c >> 1]) : Code::template pair<0, 1>(z[0][c >> 1]);
-                        const uint32_t b1 = c & 1 ? Code::template pair<2, 3>(z[1][c >> 1]) : Code::template pair<0, 1>(z[1][c >> 1]);
+                        for (int y = 0; y < 2; ++y) {
+                            const uint32_t va[4] = {Code::template pair<0, 1>(z[0][y]), Code::template pair<2, 3>(z[0][y]),
+                                                    Code::template pair<0, 1>(z[1][y]), Code::template pair<2, 3>(z[1][y])};
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            mma16816(o[mt][4 * q + c], ph[mt], b0, b1);
-                            if constexpr (SPLIT) mma16816(o[mt][4 * q + c], pl[mt], b0, b1);
+                            for (int nb = 0; nb < NB; ++nb) {
+                                mma16816(o[nb][2 * q + y], va, ph[gr][nb].x, ph[gr][nb].y);
+                                if constexpr (SPLIT) mma16816(o[nb][2 * q + y], va, pl[gr][nb].x, pl[gr][nb].y);
+                            }
                         }
                     }
                 }
@@ -650,96 +648,95 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
 
         // ---- the four warps' parts into one: each scaled to the common maximum, then added in order
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 1);
-                l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 2);
-                if (t == 0) sm.ml[warp][16 * mt + 8 * u + g] = make_float2(m[mt][u], l[mt][u]);
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
+                if (g == 0) sm.ml[warp][8 * nb + 2 * t + c] = make_float2(m[nb][c], l[nb][c]);
             }
         named_sync(1, 32 * WARPS);
-        float mt_m[MT][2], mt_l[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int c = 0; c < 2; ++c) {
                 float big = -INFINITY, sum = 0.f;
                 float2 e[WARPS];
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) {
-                    e[w] = sm.ml[w][16 * mt + 8 * u + g];
+                    e[w] = sm.ml[w][8 * nb + 2 * t + c];
                     big = fmaxf(big, e[w].x);
                 }
                 const float ref = big == -INFINITY ? 0.f : big;
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) sum += e[w].y * ex2(e[w].x - ref);
-                const float r = ex2(m[mt][u] - ref) * unit * (Code::VALUE / W_UP);
-                mt_m[mt][u] = big;
-                mt_l[mt][u] = sum;
+                const float r = ex2(m[nb][c] - ref) * unit * (Code::VALUE / W_UP);
+                m[nb][c] = big;
+                l[nb][c] = sum;
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    o[mt][j][2 * u] *= r;
-                    o[mt][j][2 * u + 1] *= r;
+                for (int j = 0; j < NJ; ++j) {
+                    o[nb][j][c] *= r;
+                    o[nb][j][2 + c] *= r;
                 }
             }
-        // Warps 2, 3 hand theirs to 0, 1, then 1 to 0.
+        // The upper half of the warps hands its part to the lower, until warp 0 has all.
 #pragma unroll
-        for (int half = 2; half >= 1; half >>= 1) {
+        for (int half = WARPS / 2; half >= 1; half >>= 1) {
             if (warp >= half && warp < 2 * half) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        sm.o[warp - half][(mt * NT + j) * 32 + lane] =
-                            make_float4(o[mt][j][0], o[mt][j][1], o[mt][j][2], o[mt][j][3]);
+                    for (int j = 0; j < NJ; ++j)
+                        sm.o[warp - half][(nb * NJ + j) * 32 + lane] =
+                            make_float4(o[nb][j][0], o[nb][j][1], o[nb][j][2], o[nb][j][3]);
             }
             named_sync(1, 32 * WARPS);
             if (warp < half) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const float4 y = sm.o[warp][(mt * NT + j) * 32 + lane];
-                        o[mt][j][0] += y.x;
-                        o[mt][j][1] += y.y;
-                        o[mt][j][2] += y.z;
-                        o[mt][j][3] += y.w;
+                    for (int j = 0; j < NJ; ++j) {
+                        const float4 y = sm.o[warp][(nb * NJ + j) * 32 + lane];
+                        o[nb][j][0] += y.x;
+                        o[nb][j][1] += y.y;
+                        o[nb][j][2] += y.z;
+                        o[nb][j][3] += y.w;
                     }
             }
-            if (half == 2) named_sync(1, 32 * WARPS);
+            if (half > 1) named_sync(1, 32 * WARPS);
         }
         if (warp == 0) {
-            // A lane's columns of rows g and g+8: 2t * VB + j from c = 0, (2t + 1) * VB + j from c = 1.
+            // Column VB g + 2j + u of row 8 nb + 2t + c is o[nb][j][2u + c].
             const bool whole = x.t0 == 0 && x.t1 == x.tiles;
             const int slot = 2 * blockIdx.x + (x.t0 == 0 ? 1 : 0);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int r = 16 * mt + 8 * u + g;
+                for (int c = 0; c < 2; ++c) {
+                    const int r = 8 * nb + 2 * t + c;
                     if (r >= rows) continue;
-                    float y[2 * VB];
-                    const float inv = whole ? (mt_l[mt][u] == 0.f ? 0.f : 1.f / mt_l[mt][u]) : 1.f;
+                    float y[VB];
+                    const float inv = whole ? (l[nb][c] == 0.f ? 0.f : 1.f / l[nb][c]) : 1.f;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) y[c * VB + j] = o[mt][j][2 * u + c] * inv;
+                        for (int u = 0; u < 2; ++u) y[2 * j + u] = o[nb][j][2 * u + c] * inv;
                     if (whole) {
                         const int h = x.hk * p.G + (x.row0 + r) % p.G;
-                        const long row = x.q0 + token[mt][u];
-                        store_out<2 * VB>(a, row * a.ld_o + h * D + 2 * VB * t, y);
-                        if (t == 0)
+                        const long row = x.q0 + (x.row0 + r) / p.G;
+                        store_out<VB>(a, row * a.ld_o + h * D + VB * g, y);
+                        if (g == 0)
                             a.lse[static_cast<long>(h) * b.N + row] =
-                                mt_l[mt][u] == 0.f ? -INFINITY : (mt_m[mt][u] + log2f(mt_l[mt][u])) * kLn2;
+                                l[nb][c] == 0.f ? -INFINITY : (m[nb][c] + log2f(l[nb][c])) * kLn2;
                     } else {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + 2 * VB * t);
+                        float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + VB * g);
 #pragma unroll
-                        for (int q = 0; q < VB / 2; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-                        if (t == 0) p.part_ml[static_cast<long>(slot) * MR + r] = make_float2(mt_m[mt][u], mt_l[mt][u]);
+                        for (int q = 0; q < VB / 4; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+                        if (g == 0) p.part_ml[static_cast<long>(slot) * MR + r] = make_float2(m[nb][c], l[nb][c]);
                     }
                 }
             if (lane == 0 && x.t0 > 0 && x.t1 == x.tiles)
-                p.joins[blockIdx.x] = Join{line.owner(x.start), x.row0, rows, x.q0, x.hk};
+                p.joins[blockIdx.x] = Join{line.owner(x.first), x.row0, rows, x.q0, x.hk};
         }
     }
 }
@@ -810,11 +807,11 @@ __global__ void __launch_bounds__(128) cached_join(const __grid_constant__ Param
     if (lane == 0) a.lse[static_cast<long>(h) * a.cache.N + at] = l == 0.f ? -INFINITY : (big + log2f(l)) * kLn2;
 }
 
-template <int D, int FORMAT, int MT, bool SPLIT>
+template <int D, int FORMAT, int NB, bool SPLIT>
 cudaError_t launch(Params& p, int ctas, bool join, cudaStream_t stream, int* launches) {
-    constexpr size_t smem = sizeof(Smem<D, MT, SPLIT>) + 1024;
+    constexpr size_t smem = sizeof(Smem<D, NB, SPLIT>) + 1024;
     static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs to an SM");
-    auto kernel = cached_fwd<D, FORMAT, MT, SPLIT>;
+    auto kernel = cached_fwd<D, FORMAT, NB, SPLIT>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -829,7 +826,7 @@ cudaError_t launch(Params& p, int ctas, bool join, cudaStream_t stream, int* lau
     if (e != cudaSuccess) return e;
     ++*launches;
     if (!join) return cudaSuccess;
-    e = launch_pdl(cached_join<D, 16 * MT>, dim3(ctas, 4 * MT), dim3(128), 0, stream, p);
+    e = launch_pdl(cached_join<D, 8 * NB>, dim3(ctas, 2 * NB), dim3(128), 0, stream, p);
     if (e == cudaSuccess) ++*launches;
     return e;
 }
@@ -843,10 +840,11 @@ ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, 
     p.a = a;
     p.page_shift = page_shift_of(b.c.page_size);
     p.G = a.H / b.c.n_kv_head;
-    // Row tiles of 32 where the batch has more than 16 rows to a key head on average: they read the cache
-    // half as often; smaller ones leave more registers and half the idle rows.
-    const int MT = static_cast<long>(b.N) * p.G > 16L * b.S ? 2 : 1;
-    const int MR = 16 * MT, ctas = 2 * num_sms;
+    // Row tiles of 8, 16 or 32, the smallest that holds a sequence's rows on average: fewer row tiles read
+    // the cache less often, smaller ones leave fewer idle rows.
+    const long per_seq = (static_cast<long>(b.N) * p.G + b.S - 1) / b.S;
+    const int NB = per_seq <= 8 ? 1 : per_seq <= 16 ? 2 : 4;
+    const int MR = 8 * NB, ctas = 2 * num_sms;
     const bool join = (static_cast<long>(b.max_pages) << p.page_shift) > TK;  // else no item has two tiles
     ProjStatus st;
     const size_t o_bytes = sizeof(float) * 2 * ctas * MR * D, ml_bytes = sizeof(float2) * 2 * ctas * MR;
@@ -868,20 +866,21 @@ ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, 
             st.cuda = cudaErrorInvalidValue;
     }
     if (st.ok()) {
-        auto pick = [&](auto d, auto fmt, auto mt, auto split) {
-            return launch<decltype(d)::value, decltype(fmt)::value, decltype(mt)::value, decltype(split)::value>(
+        auto pick = [&](auto d, auto fmt, auto nb, auto split) {
+            return launch<decltype(d)::value, decltype(fmt)::value, decltype(nb)::value, decltype(split)::value>(
                 p, ctas, join, s, launches);
         };
-        auto by_split = [&](auto d, auto fmt, auto mt) {
-            return a.dtype == KATTN_F32 ? pick(d, fmt, mt, std::true_type{}) : pick(d, fmt, mt, std::false_type{});
+        auto by_split = [&](auto d, auto fmt, auto nb) {
+            return a.dtype == KATTN_F32 ? pick(d, fmt, nb, std::true_type{}) : pick(d, fmt, nb, std::false_type{});
         };
-        auto by_mt = [&](auto d, auto fmt) {
-            return MT == 1 ? by_split(d, fmt, std::integral_constant<int, 1>{})
-                           : by_split(d, fmt, std::integral_constant<int, 2>{});
+        auto by_nb = [&](auto d, auto fmt) {
+            return NB == 1   ? by_split(d, fmt, std::integral_constant<int, 1>{})
+                   : NB == 2 ? by_split(d, fmt, std::integral_constant<int, 2>{})
+                             : by_split(d, fmt, std::integral_constant<int, 4>{});
         };
         auto by_format = [&](auto d) {
-            return b.c.format == KATTN_CACHE_INT8 ? by_mt(d, std::integral_constant<int, KATTN_CACHE_INT8>{})
-                                                  : by_mt(d, std::integral_constant<int, KATTN_CACHE_E4M3>{});
+            return b.c.format == KATTN_CACHE_INT8 ? by_nb(d, std::integral_constant<int, KATTN_CACHE_INT8>{})
+                                                  : by_nb(d, std::integral_constant<int, KATTN_CACHE_E4M3>{});
         };
         st.cuda = D == 32   ? by_format(std::integral_constant<int, 32>{})
                   : D == 64 ? by_format(std::integral_constant<int, 64>{})
