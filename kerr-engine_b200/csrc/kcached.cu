@@ -79,7 +79,7 @@ struct Cfg {
     static constexpr int GR = NB > 2 ? 1 : 2;                  // groups of 16 positions a warp takes at once
     static constexpr bool Q_SMEM = NB * D * (SPLIT ? 2 : 1) > 256;  // q in shared memory rather than registers
     static constexpr int Q_WORDS = Q_SMEM ? KS * NB * (SPLIT ? 2 : 1) * 32 : 1;
-    static constexpr int FIT = (106 * 1024 - WARPS / 2 * MR * D * 4 - 8 * Q_WORDS) / (2 * TK * (D + 4));
+    static constexpr int FIT = (111 * 1024 + 512 - WARPS / 2 * MR * D * 4 - 8 * Q_WORDS) / (2 * TK * (D + 4));
     static constexpr int STAGES = FIT < 6 ? FIT : 6;
 };
 
@@ -142,7 +142,7 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
 // arrive through prepare(), one word of four.
 template <int FORMAT>
 struct Codes {
-    static constexpr float VALUE = FORMAT == KATTN_CACHE_INT8 ? 1.f : 256.f;  // of a converted code's one
+    static constexpr float VALUE = 1.f;
     static __device__ __forceinline__ uint32_t prepare(uint32_t w) {
         return FORMAT == KATTN_CACHE_INT8 ? w ^ 0x80808080u : w;
     }
@@ -152,8 +152,11 @@ struct Codes {
         if constexpr (FORMAT == KATTN_CACHE_INT8) {
             return sub2(prmt(w, 0x64646464u, 0x4040u | I | (J << 8)), 0x64806480u);
         } else {
-            const uint32_t x = prmt(w, 0u, 0x0404u | (I << 4) | (J << 12));
-            return (x & 0x80008000u) | ((x >> 1) & 0x3F803F80u);
+            static_assert(J == I + 1 && I % 2 == 0, "a half of the word");
+            uint32_t x;
+            const uint16_t two = static_cast<uint16_t>(I == 0 ? w : w >> 16);
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(x) : "h"(two));
+            return x;
         }
     }
 };
@@ -617,6 +620,11 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                                 to[0] = w.x, to[1] = w.y;
                             } else {
                                 to[0] = *reinterpret_cast<const uint32_t*>(vt + chunk_at<D>(r, g >> 2) + 4 * (g & 3));
+                            }
+                            // A place that no position has may hold e4m3's NaN, which a weight of zero does not remove.
+                            if (FORMAT == KATTN_CACHE_E4M3 && !seen_all && (pos0 + r >= x.len || !((here >> gr) & 1))) {
+#pragma unroll
+                                for (int q = 0; q < VB / 4; ++q) to[q] = 0;
                             }
                         }
 #pragma unroll
