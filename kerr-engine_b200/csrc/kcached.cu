@@ -20,7 +20,7 @@
 // (two to an SM), whatever the lengths; an item cut by a border leaves parts
 // (row maxima, sums, O) in a workspace, which cached_join adds in order.
 //
-// Operands.  Codes are exact in f16 (int8 as they are, e4m3 times 2^-8), so
+// Operands.  Codes are exact in f16, so
 // only q and the weights are rounded: q to f16 after a power of two per row has
 // brought its largest element near 2^13 (exact for bf16 and f16 but for elements 2^-37
 // of it; f32 as a hi / lo pair), the weights p_j vs_j to f16 after a power of two
@@ -49,11 +49,14 @@ using namespace sm100;
 
 constexpr int TK = 128;              // positions of a tile
 constexpr int WARPS = 4;             // computing warps, 32 positions of a tile each
-// A warpgroup computes and one of another issues the copies (its other warps only lend their registers): two
-// such CTAs to an SM.
-constexpr int N_THREADS = 256, R_COMPUTE = 208, R_COPY = 48;
+// A warpgroup computes; of the other, a warp walks the line of work and issues the copies, one brings q into shared
+// memory, one writes results (so an item's start and end cost the computing warps little), and registers are lent.
+// Two such CTAs to an SM.
+constexpr int N_THREADS = 256, R_COMPUTE = 208, R_SERVE = 48;
+constexpr int COPY_WARP = WARPS, Q_WARP = WARPS + 1, OUT_WARP = WARPS + 2;
+constexpr int PIECES = 4;            // ring of pieces
 constexpr float RAISE = 8.f;         // a row's reference is raised when its maximum passes it by 2^8
-constexpr int EXTRA = 2;             // what an item's rows, joins and stores cost, in tiles
+constexpr int EXTRA = 1;             // what an item's rows, joins and stores cost, in tiles
 constexpr float W_UP = 128.f;        // weights are held times 2^7: at most 2^15 with RAISE, far from f16's subnormals
 
 // A part's place in the line of work, and what joins it.
@@ -78,9 +81,21 @@ struct Cfg {
     static constexpr int KS = D / 16;                          // k steps of the first product
     static constexpr int GR = NB > 2 ? 1 : 2;                  // groups of 16 positions a warp takes at once
     static constexpr bool Q_SMEM = NB * D * (SPLIT ? 2 : 1) > 256;  // q in shared memory rather than registers
-    static constexpr int Q_WORDS = Q_SMEM ? KS * NB * (SPLIT ? 2 : 1) * 32 : 1;
-    static constexpr int FIT = (111 * 1024 + 512 - WARPS / 2 * MR * D * 4 - 8 * Q_WORDS) / (2 * TK * (D + 4));
+    static constexpr int Q_WORDS = KS * NB * (SPLIT ? 2 : 1) * 32;  // of a piece
+    static constexpr int Q_SLOTS = Q_WORDS >= 1024 ? 1 : 2;
+    static constexpr int FIT = (110 * 1024 - WARPS / 2 * MR * D * 4 - 8 * Q_WORDS * Q_SLOTS) / (2 * TK * (D + 4));
     static constexpr int STAGES = FIT < 6 ? FIT : 6;
+    static_assert(STAGES >= 2, "stages");
+};
+
+// A stretch of an item's tiles.
+struct Piece {
+    int s, q0, n, len;   // sequence, its first row, rows and length
+    int base;            // the first new position
+    int hk, row0, rows;  // key head, first row of the row tile and how many
+    int t0, t1, tiles;   // its tiles t0 .. t1-1 of the item's
+    int first_cta;       // the CTA of the item's first tile
+    int valid;
 };
 
 template <int D, int NB, bool SPLIT>
@@ -90,11 +105,17 @@ struct Smem {
     alignas(1024) uint8_t v[C::STAGES][TK * D];
     alignas(16) float ks[C::STAGES][TK];
     alignas(16) float vs[C::STAGES][TK];
-    alignas(16) uint2 q[C::Q_WORDS];
-    alignas(16) float4 o[WARPS / 2][C::MR * D / 4];  // O of half the warps, handed to the other
-    float2 ml[WARPS][C::MR];
+    alignas(16) uint2 q[C::Q_SLOTS][C::Q_WORDS];
+    alignas(16) float4 o[WARPS / 2][C::MR * D / 4];  // the warps' O on its way to one
+    float f[C::Q_SLOTS][C::MR];                      // factors of the rows' scores
+    float2 ml[WARPS][C::MR];                         // the warps' row maxima and sums
+    float2 row[C::MR];                               // the piece's
+    Piece pieces[PIECES];
     uint32_t valid[C::STAGES];  // a bit for each 16 positions: they exist
     uint64_t full[C::STAGES], empty[C::STAGES];
+    uint64_t piece_full[PIECES], piece_empty[PIECES];
+    uint64_t q_full[C::Q_SLOTS], q_empty[C::Q_SLOTS];
+    uint64_t meet, o_full, o_empty;
 };
 
 // The position, of 8, behind column n = 2t + b of an n8 tile.
@@ -138,11 +159,9 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
 }
 
 // Codes as f16 pairs.  int8: code + 128 under 1024's exponent is 1152 + code.
-// e4m3: its exponent and mantissa under f16's, the number times 2^-8.  Codes
-// arrive through prepare(), one word of four.
+// e4m3 has an instruction.  Codes arrive through prepare(), one word of four.
 template <int FORMAT>
 struct Codes {
-    static constexpr float VALUE = 1.f;
     static __device__ __forceinline__ uint32_t prepare(uint32_t w) {
         return FORMAT == KATTN_CACHE_INT8 ? w ^ 0x80808080u : w;
     }
@@ -162,13 +181,6 @@ struct Codes {
 };
 
 // ---------------------------------------------------------------- the line of work
-struct Piece {
-    int s, q0, n, len;   // sequence, its first row, rows and length
-    int hk, row0;        // key head, first row of the row tile
-    int t0, t1, tiles;   // its tiles t0 .. t1-1 of the item's
-    long first;          // the place of its first tile in the line
-};
-
 // An item counts EXTRA tiles before its own.
 template <int MR>
 struct Line {
@@ -239,11 +251,14 @@ struct Line {
             p.len = len;
             p.hk = item / row_tiles;
             p.row0 = (item % row_tiles) * MR;
+            p.rows = min(n * G - p.row0, MR);
+            p.base = max(__ldg(a.cache.kv_len + s), 0) - n;
             p.tiles = tiles;
-            p.first = base + static_cast<long>(item) * (tiles + EXTRA) + EXTRA;
-            p.t0 = static_cast<int>(max(at - p.first, 0L));
-            p.t1 = static_cast<int>(min(static_cast<long>(tiles), end - p.first));
-            at = p.first + p.t1;
+            const long first = base + static_cast<long>(item) * (tiles + EXTRA) + EXTRA;  // the place of its first tile
+            p.t0 = static_cast<int>(max(at - first, 0L));
+            p.t1 = static_cast<int>(min(static_cast<long>(tiles), end - first));
+            p.first_cta = owner(first);
+            at = first + p.t1;
             if (p.t1 > p.t0) return true;
             at = end;  // the border lies before the item's first tile
         }
@@ -302,74 +317,216 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     pdl_launch();
     if (tid == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(&sm.full[i], 33);  // the copy's issuer and every lane's scales
+            mbar_init(&sm.full[i], 33);  // the copies' issuer and every lane's scales
             mbar_init(&sm.empty[i], WARPS);
         }
+        for (int i = 0; i < PIECES; ++i) {
+            mbar_init(&sm.piece_full[i], 1);
+            mbar_init(&sm.piece_empty[i], WARPS + 2);
+        }
+        for (int i = 0; i < C::Q_SLOTS; ++i) {
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], WARPS);
+        }
+        mbar_init(&sm.meet, WARPS);
+        mbar_init(&sm.o_full, 2);
+        mbar_init(&sm.o_empty, 1);
         fence_barrier_init();
     }
     __syncthreads();
     pdl_wait();
 
-    const int capacity = static_cast<int>(min(static_cast<long>(b.max_pages) << p.page_shift, 0x7FFFFFC0L));
-    Line<MR> line{a, p.G, lane, capacity};
-    const bool any = line.start(blockIdx.x, gridDim.x);
-    if (tid == 0) p.joins[blockIdx.x].first_cta = -1;
-    if (!any) return;
-    Piece x;
-    int st = 0, turn = 0;  // ring
+    // A wait that runs out sets the status word, and the warp leaves; the others' waits then run out too.
+    auto await = [&](uint64_t* bar, uint32_t parity) {
+        const bool ok = mbar_wait_warp(bar, parity, a.wait_ns);
+        if (!ok && lane == 0) atomicOr(a.status, 1);
+        return ok;
+    };
+    auto arrive = [&](uint64_t* bar) {  // once for the warp
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    const Piece* piece = nullptr;
+    auto next_piece = [&](int i) {  // the i-th, for a warp that reads them
+        if (!await(&sm.piece_full[i % PIECES], (i / PIECES) & 1)) return false;
+        piece = &sm.pieces[i % PIECES];
+        return piece->valid != 0;
+    };
 
     if (warp >= WARPS) {
-        // ------------------------------------------------------------ copies
-        regs_dec<R_COPY>();
-        if (warp > WARPS) return;
-        const int frag_shift = min(p.page_shift, 7);  // a tile is TK >> frag_shift stretches of a page
-        const int frags = TK >> frag_shift, frag = 1 << frag_shift;
-        if (lane == 0 && b.c.n_pages > 0 && b.max_pages > 0) {
-            prefetch_tensormap(&p.tk);
-            prefetch_tensormap(&p.tv);
-        }
-        while (line.next(x)) {
-            const int s = x.s;
-            for (int i = x.t0; i < x.t1; ++i) {
-                const int pos = i * TK + lane * frag;
-                int page = -1;
-                if (lane < frags && pos < x.len) page = page_of(b, p.page_shift, s, pos);
-                const unsigned ok = __ballot_sync(0xffffffffu, page >= 0);
-                if (turn > 0 && !mbar_wait_warp(&sm.empty[st], (turn - 1) & 1, a.wait_ns)) {
-                    // Copies still landing complete before the shared memory is released.
-                    for (int f = 0; f < C::STAGES; ++f) {
-                        mbar_wait(&sm.full[st], (turn - 1) & 1, 10000000ull);
-                        if (++st == C::STAGES) st = 0, ++turn;
-                    }
-                    if (lane == 0) atomicOr(a.status, 1);
-                    return;
-                }
+        regs_dec<R_SERVE>();
+        if (warp == COPY_WARP) {
+            // -------------------------------------------------------- the line of work, copies
+            if (tid == 32 * COPY_WARP) p.joins[blockIdx.x].first_cta = -1;
+            if (lane == 0 && b.c.n_pages > 0 && b.max_pages > 0) {
+                prefetch_tensormap(&p.tk);
+                prefetch_tensormap(&p.tv);
+            }
+            const int capacity = static_cast<int>(min(static_cast<long>(b.max_pages) << p.page_shift, 0x7FFFFFC0L));
+            Line<MR> line{a, p.G, lane, capacity};
+            const int frag_shift = min(p.page_shift, 7), frag = 1 << frag_shift;  // a stretch of a page that a copy takes
+            bool more = line.start(blockIdx.x, gridDim.x);
+            int st = 0, turn = 0;
+            for (int i = 0;; ++i) {
+                Piece x;
+                more = more && line.next(x);
+                x.valid = more;
+                if (i >= PIECES && !await(&sm.piece_empty[i % PIECES], (i / PIECES - 1) & 1)) break;
                 if (lane == 0) {
-                    uint32_t bits = 0;
-                    for (int f = 0; f < frags; ++f)
-                        if ((ok >> f) & 1) bits |= ((1u << (frag >> 4)) - 1u) << (f * (frag >> 4));
-                    sm.valid[st] = bits;
-                    mbar_arrive_expect_tx(&sm.full[st], __popc(ok) * 2 * frag * D);
+                    sm.pieces[i % PIECES] = x;
+                    mbar_arrive(&sm.piece_full[i % PIECES]);
                 }
-                __syncwarp();
-                const int in_page = pos & (b.c.page_size - 1);
-                if (page >= 0) {
-                    const int row = (x.hk << p.page_shift) + in_page;
-                    tma_load_3d(sm.k[st] + lane * frag * D, &p.tk, 0, row, page, &sm.full[st]);
-                    tma_load_3d(sm.v[st] + lane * frag * D, &p.tv, 0, row, page, &sm.full[st]);
+                if (!more) return;
+                // Lane f looks up the page of the f-th stretch, a tile ahead.
+                auto page_at = [&](int tile) {
+                    const int pos = tile * TK + lane * frag;
+                    return lane < (TK >> frag_shift) && pos < x.len ? page_of(b, p.page_shift, x.s, pos) : -1;
+                };
+                int next = page_at(x.t0);
+                bool ok = true;
+                for (int j = x.t0; j < x.t1; ++j) {
+                    const int page = next;
+                    if (j + 1 < x.t1) next = page_at(j + 1);
+                    const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+                    const int page16 = __shfl_sync(0xffffffffu, page, ((lane & 7) * 16) >> frag_shift);
+                    const unsigned bits = __ballot_sync(0xffffffffu, page16 >= 0) & 0xFFu;
+                    const int page4 = __shfl_sync(0xffffffffu, page, (lane * 4) >> frag_shift);
+                    if (turn > 0 && !await(&sm.empty[st], (turn - 1) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        sm.valid[st] = bits;
+                        mbar_arrive_expect_tx(&sm.full[st], __popc(there) * 2 * frag * D);
+                    }
+                    __syncwarp();
+                    if (page >= 0) {
+                        const int row = (x.hk << p.page_shift) + ((j * TK + lane * frag) & (b.c.page_size - 1));
+                        tma_load_3d(sm.k[st] + lane * frag * D, &p.tk, 0, row, page, &sm.full[st]);
+                        tma_load_3d(sm.v[st] + lane * frag * D, &p.tv, 0, row, page, &sm.full[st]);
+                    }
+                    if (page4 >= 0) {  // scales, four of each a lane
+                        const long row = ((static_cast<long>(page4) * b.c.n_kv_head + x.hk) << p.page_shift) +
+                                         ((j * TK + lane * 4) & (b.c.page_size - 1));
+                        cp_async16(&sm.ks[st][lane * 4], b.c.k_scale + row, 16);
+                        cp_async16(&sm.vs[st][lane * 4], b.c.v_scale + row, 16);
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[st]))
+                                 : "memory");
+                    if (++st == C::STAGES) st = 0, ++turn;
                 }
-                // Scales, four of each a lane.
-                const int c4 = lane * 4;
-                const int page4 = __shfl_sync(0xffffffffu, page, c4 >> frag_shift);
-                if (page4 >= 0) {
-                    const long row = ((static_cast<long>(page4) * b.c.n_kv_head + x.hk) << p.page_shift) +
-                                     ((i * TK + c4) & (b.c.page_size - 1));
-                    cp_async16(&sm.ks[st][c4], b.c.k_scale + row, 16);
-                    cp_async16(&sm.vs[st][c4], b.c.v_scale + row, 16);
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&sm.full[st]))
-                             : "memory");
+                if (!ok) break;
+            }
+            // After a wait that ran out: copies still landing complete before the shared memory is released.
+            for (int f = 0; f < C::STAGES; ++f) {
+                if (turn > 0) mbar_wait(&sm.full[st], (turn - 1) & 1, 10000000ull);
                 if (++st == C::STAGES) st = 0, ++turn;
+            }
+        } else if (warp == Q_WARP) {
+            // -------------------------------------------------------- q
+            // Operand B, row 8 nb + g: k slots (2t, 2t+1) and (2t+8, 2t+9) of step k are four neighbouring columns.
+            for (int i = 0; next_piece(i); ++i) {
+                const int slot = i % C::Q_SLOTS, use = i / C::Q_SLOTS;
+                if (use > 0 && !await(&sm.q_empty[slot], (use - 1) & 1)) return;
+#pragma unroll 1
+                for (int nb = 0; nb < NB; ++nb) {
+                    const int r = 8 * nb + g, row = piece->row0 + r;
+                    const bool in = r < piece->rows;
+                    const long at = static_cast<long>(piece->q0 + row / p.G) * a.ld_q + (piece->hk * p.G + row % p.G) * D;
+                    auto four = [&](int k) {
+                        return in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                    };
+                    float most = 0.f;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const float4 w = four(k);
+                        most = fmaxf(most, fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))));
+                    }
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    // The row times 2^(13 - e), e the exponent of its largest element.
+                    const int e = most < INFINITY ? max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) : 13;
+                    const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
+                    const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
+                    if (t == 0) sm.f[slot][r] = down * (a.scale * kLog2e);
+#pragma unroll 4
+                    for (int k = 0; k < KS; ++k) {
+                        const float4 w = four(k);
+                        const float4 v = make_float4(w.x * up, w.y * up, w.z * up, w.w * up);
+                        const uint2 hi = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+                        sm.q[slot][(k * NB + nb) * 32 + lane] = hi;
+                        if constexpr (SPLIT) {
+                            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                            const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                            sm.q[slot][((KS + k) * NB + nb) * 32 + lane] =
+                                make_uint2(pack_f16(v.x - h0.x, v.y - h0.y), pack_f16(v.z - h1.x, v.w - h1.y));
+                        }
+                    }
+                }
+                arrive(&sm.q_full[slot]);
+                arrive(&sm.piece_empty[i % PIECES]);
+            }
+        } else if (warp == OUT_WARP) {
+            // -------------------------------------------------------- results
+            // Column VB g + 2j + u of row 8 nb + 2t + c is component 2u + c of o[.][nb, j].
+            for (int i = 0; next_piece(i); ++i) {
+                if (!await(&sm.o_full, i & 1)) return;
+                const Piece x = *piece;
+                const bool whole = x.t0 == 0 && x.t1 == x.tiles;
+                const int slot = 2 * blockIdx.x + (x.t0 == 0 ? 1 : 0);
+#pragma unroll 1
+                for (int nb = 0; nb < NB; ++nb) {
+                    const int r0 = 8 * nb + 2 * t;
+                    const float2 ml[2] = {sm.row[r0], sm.row[r0 + 1]};
+                    constexpr int JS = NJ < 4 ? NJ : 4;  // two columns each
+#pragma unroll 1
+                    for (int j0 = 0; j0 < NJ; j0 += JS) {
+                        float y[2][2 * JS];
+#pragma unroll
+                        for (int j = 0; j < JS; ++j) {
+                            const float4 v0 = sm.o[0][(nb * NJ + j0 + j) * 32 + lane];
+                            const float4 v1 = sm.o[1][(nb * NJ + j0 + j) * 32 + lane];
+                            y[0][2 * j] = v0.x + v1.x;
+                            y[1][2 * j] = v0.y + v1.y;
+                            y[0][2 * j + 1] = v0.z + v1.z;
+                            y[1][2 * j + 1] = v0.w + v1.w;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int r = r0 + c;
+                            if (r >= x.rows) continue;
+                            if (whole) {
+                                const int row = x.row0 + r, h = x.hk * p.G + row % p.G;
+                                const float inv = ml[c].y == 0.f ? 0.f : 1.f / ml[c].y;
+#pragma unroll
+                                for (int q = 0; q < 2 * JS; ++q) y[c][q] *= inv;
+                                store_out<2 * JS>(a, static_cast<long>(x.q0 + row / p.G) * a.ld_o + h * D + VB * g + 2 * j0, y[c]);
+                            } else {
+                                float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + VB * g + 2 * j0);
+#pragma unroll
+                                for (int q = 0; q < JS / 2; ++q)
+                                    dst[q] = make_float4(y[c][4 * q], y[c][4 * q + 1], y[c][4 * q + 2], y[c][4 * q + 3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int r = r0 + c;
+                        if (g != 0 || r >= x.rows) continue;
+                        if (whole) {
+                            const int row = x.row0 + r, h = x.hk * p.G + row % p.G;
+                            a.lse[static_cast<long>(h) * b.N + x.q0 + row / p.G] =
+                                ml[c].y == 0.f ? -INFINITY : (ml[c].x + log2f(ml[c].y)) * kLn2;
+                        } else {
+                            p.part_ml[static_cast<long>(slot) * MR + r] = ml[c];
+                        }
+                    }
+                }
+                if (lane == 0 && x.t0 > 0 && x.t1 == x.tiles)
+                    p.joins[blockIdx.x] = Join{x.first_cta, x.row0, x.rows, x.q0, x.hk};
+                arrive(&sm.o_empty);
+                arrive(&sm.piece_empty[i % PIECES]);
             }
         }
         return;
@@ -378,59 +535,28 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     // ---------------------------------------------------------------- products
     regs_inc<R_COMPUTE>();
     // This lane's rows are 8 nb + 2t + c; the statistics of a row are the same in its eight lanes.
-    bool dead = false;
-    while (line.next(x)) {
-        const int rows = min(x.n * p.G - x.row0, MR);
-        const int base = max(__ldg(b.kv_len + x.s), 0) - x.n;  // the first new position
-        // q as operand B, row 8 nb + g: k slots (2t, 2t+1) and (2t+8, 2t+9) of step k are four neighbouring columns.
+    int st = 0, turn = 0;  // ring of tiles
+    uint32_t met = 0;      // meetings of the computing warps, their parity
+    for (int i = 0; next_piece(i); ++i) {
+        const int row0 = piece->row0, rows = piece->rows, base = piece->base, len = piece->len, q0 = piece->q0;
+        const int t0 = piece->t0, t1 = piece->t1;
+        const int slot = i % C::Q_SLOTS;
+        if (!await(&sm.q_full[slot], (i / C::Q_SLOTS) & 1)) return;
         uint2 qh[C::Q_SMEM ? 1 : KS][NB], ql[SPLIT && !C::Q_SMEM ? KS : 1][NB];
         float f[NB][2];  // factors of the rows' scores
-        if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);  // the piece before is done with q
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int r = 8 * nb + g, row = x.row0 + r;
-            const bool in = r < rows;
-            const long at = static_cast<long>(x.q0 + row / p.G) * a.ld_q + (x.hk * p.G + row % p.G) * D;
-            float4 w[KS];
-            float most = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                w[k] = in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-                most = fmaxf(most, fmaxf(fmaxf(fabsf(w[k].x), fabsf(w[k].y)), fmaxf(fabsf(w[k].z), fabsf(w[k].w))));
-            }
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            // The row times 2^(13 - e), e the exponent of its largest element.
-            const int e = most < INFINITY ? max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100) : 13;
-            const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
-            const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
+            for (int c = 0; c < 2; ++c) f[nb][c] = sm.f[slot][8 * nb + 2 * t + c];
+            if constexpr (!C::Q_SMEM) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f[nb][c] = __shfl_sync(0xffffffffu, down, (2 * t + c) * 4) * (a.scale * kLog2e) * Code::VALUE;
-            }
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const float4 v = make_float4(w[k].x * up, w[k].y * up, w[k].z * up, w[k].w * up);
-                const uint2 hi = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
-                uint2 lo = make_uint2(0, 0);
-                if constexpr (SPLIT) {
-                    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-                    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-                    lo = make_uint2(pack_f16(v.x - h0.x, v.y - h0.y), pack_f16(v.z - h1.x, v.w - h1.y));
-                }
-                if constexpr (C::Q_SMEM) {
-                    if (warp == nb % WARPS) {
-                        sm.q[(k * NB + nb) * 32 + lane] = hi;
-                        if constexpr (SPLIT) sm.q[((KS + k) * NB + nb) * 32 + lane] = lo;
-                    }
-                } else {
-                    qh[k][nb] = hi;
-                    if constexpr (SPLIT) ql[k][nb] = lo;
+                for (int k = 0; k < KS; ++k) {
+                    qh[k][nb] = sm.q[slot][(k * NB + nb) * 32 + lane];
+                    if constexpr (SPLIT) ql[k][nb] = sm.q[slot][((KS + k) * NB + nb) * 32 + lane];
                 }
             }
         }
-        if constexpr (C::Q_SMEM) named_sync(1, 32 * WARPS);
+        if constexpr (!C::Q_SMEM) arrive(&sm.q_empty[slot]);
 
         float o[NB][NJ][4], m[NB][2], l[NB][2];
         float unit = 0.f, w_in = 0.f;  // a power of two, at least the largest value scale so far; 2^7 / unit
@@ -444,18 +570,14 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 for (int i = 0; i < 4; ++i) o[nb][j][i] = 0.f;
         }
 
-        for (int i = x.t0; i < x.t1; ++i) {
-            // After a wait that ran out the warp goes on without waiting or computing, to the CTA's barriers and its end.
-            if (!dead && !mbar_wait_warp(&sm.full[st], turn & 1, a.wait_ns)) {
-                dead = true;
-                if (lane == 0) atomicOr(a.status, 1);
-            }
+        for (int tile = t0; tile < t1; ++tile) {
+            if (!await(&sm.full[st], turn & 1)) return;
 #pragma unroll 1
             for (int step = 0; step < 2 / GR; ++step) {
                 const int group = warp * 2 + step * GR;  // of 16 positions
-                const int pos0 = i * TK + group * 16;
+                const int pos0 = tile * TK + group * 16;
                 const uint32_t here = (sm.valid[st] >> group) & ((1u << GR) - 1u);
-                if (dead || here == 0 || pos0 >= x.len) continue;
+                if (here == 0 || pos0 >= len) continue;
                 const uint8_t* kt = sm.k[st] + group * 16 * D;
                 const uint8_t* vt = sm.v[st] + group * 16 * D;
                 // ---- S^T = codes of K . q
@@ -492,17 +614,17 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                                                 Code::template pair<2, 3>(w0), Code::template pair<2, 3>(w1)};
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            const uint2 h = C::Q_SMEM ? sm.q[(k * NB + nb) * 32 + lane] : qh[C::Q_SMEM ? 0 : k][nb];
+                            const uint2 h = C::Q_SMEM ? sm.q[slot][(k * NB + nb) * 32 + lane] : qh[C::Q_SMEM ? 0 : k][nb];
                             mma16816(s[gr][nb], ka, h.x, h.y);
                             if constexpr (SPLIT) {
-                                const uint2 e = C::Q_SMEM ? sm.q[((KS + k) * NB + nb) * 32 + lane] : ql[C::Q_SMEM ? 0 : k][nb];
+                                const uint2 e = C::Q_SMEM ? sm.q[slot][((KS + k) * NB + nb) * 32 + lane] : ql[C::Q_SMEM ? 0 : k][nb];
                                 mma16816(s[gr][nb], ka, e.x, e.y);
                             }
                         }
                     }
                 }
                 // ---- scores and masks
-                const bool seen_all = pos0 + 16 * GR <= min(base, x.len) && here == (1u << GR) - 1u;
+                const bool seen_all = pos0 + 16 * GR <= min(base, len) && here == (1u << GR) - 1u;
                 float vs[GR][2];
                 bool raise = false;
 #pragma unroll
@@ -518,16 +640,16 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                             for (int c = 0; c < 2; ++c) s[gr][nb][2 * u + c] *= k_s * f[nb][c];
                         if (!seen_all) {
                             const int pos = pos0 + r, j = pos - base;  // j: the place among the new tokens
-                            const bool exists = pos < x.len && ((here >> gr) & 1);
+                            const bool exists = pos < len && ((here >> gr) & 1);
                             if (!exists) vs[gr][u] = 0.f;
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    const int mine = 8 * nb + 2 * t + c, token = (x.row0 + mine) / p.G;
+                                    const int mine = 8 * nb + 2 * t + c, token = (row0 + mine) / p.G;
                                     bool see = exists && mine < rows;
                                     if (see && j >= 0)
-                                        see = a.tree ? j < 64 && ((__ldg(a.tree + x.q0 + token) >> j) & 1) : j <= token;
+                                        see = a.tree ? j < 64 && ((__ldg(a.tree + q0 + token) >> j) & 1) : j <= token;
                                     if (!see) s[gr][nb][2 * u + c] = -INFINITY;
                                 }
                         }
@@ -622,7 +744,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                                 to[0] = *reinterpret_cast<const uint32_t*>(vt + chunk_at<D>(r, g >> 2) + 4 * (g & 3));
                             }
                             // A place that no position has may hold e4m3's NaN, which a weight of zero does not remove.
-                            if (FORMAT == KATTN_CACHE_E4M3 && !seen_all && (pos0 + r >= x.len || !((here >> gr) & 1))) {
+                            if (FORMAT == KATTN_CACHE_E4M3 && !seen_all && (pos0 + r >= len || !((here >> gr) & 1))) {
 #pragma unroll
                                 for (int q = 0; q < VB / 4; ++q) to[q] = 0;
                             }
@@ -649,10 +771,10 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.empty[st]);
+            arrive(&sm.empty[st]);
             if (++st == C::STAGES) st = 0, ++turn;
         }
+        if constexpr (C::Q_SMEM) arrive(&sm.q_empty[slot]);
 
         // ---- the four warps' parts into one: each scaled to the common maximum, then added in order
 #pragma unroll
@@ -663,7 +785,9 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
                 if (g == 0) sm.ml[warp][8 * nb + 2 * t + c] = make_float2(m[nb][c], l[nb][c]);
             }
-        named_sync(1, 32 * WARPS);
+        arrive(&sm.meet);
+        if (!await(&sm.meet, met)) return;
+        met ^= 1;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -678,7 +802,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 const float ref = big == -INFINITY ? 0.f : big;
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) sum += e[w].y * ex2(e[w].x - ref);
-                const float r = ex2(m[nb][c] - ref) * unit * (Code::VALUE / W_UP);
+                const float r = ex2(m[nb][c] - ref) * unit * (1.f / W_UP);
                 m[nb][c] = big;
                 l[nb][c] = sum;
 #pragma unroll
@@ -687,65 +811,39 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                     o[nb][j][2 + c] *= r;
                 }
             }
-        // The upper half of the warps hands its part to the lower, until warp 0 has all.
-#pragma unroll
-        for (int half = WARPS / 2; half >= 1; half >>= 1) {
-            if (warp >= half && warp < 2 * half) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-                        sm.o[warp - half][(nb * NJ + j) * 32 + lane] =
-                            make_float4(o[nb][j][0], o[nb][j][1], o[nb][j][2], o[nb][j][3]);
-            }
-            named_sync(1, 32 * WARPS);
-            if (warp < half) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        const float4 y = sm.o[warp][(nb * NJ + j) * 32 + lane];
-                        o[nb][j][0] += y.x;
-                        o[nb][j][1] += y.y;
-                        o[nb][j][2] += y.z;
-                        o[nb][j][3] += y.w;
-                    }
-            }
-            if (half > 1) named_sync(1, 32 * WARPS);
-        }
-        if (warp == 0) {
-            // Column VB g + 2j + u of row 8 nb + 2t + c is o[nb][j][2u + c].
-            const bool whole = x.t0 == 0 && x.t1 == x.tiles;
-            const int slot = 2 * blockIdx.x + (x.t0 == 0 ? 1 : 0);
+        // Warps 2 and 3 hand theirs to 0 and 1, whose sums the result warp adds.
+        if (i > 0 && !await(&sm.o_empty, (i - 1) & 1)) return;
+        float4* mine = sm.o[warp & 1];
+        if (warp >= 2) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int r = 8 * nb + 2 * t + c;
-                    if (r >= rows) continue;
-                    float y[VB];
-                    const float inv = whole ? (l[nb][c] == 0.f ? 0.f : 1.f / l[nb][c]) : 1.f;
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) y[2 * j + u] = o[nb][j][2 * u + c] * inv;
-                    if (whole) {
-                        const int h = x.hk * p.G + (x.row0 + r) % p.G;
-                        const long row = x.q0 + (x.row0 + r) / p.G;
-                        store_out<VB>(a, row * a.ld_o + h * D + VB * g, y);
-                        if (g == 0)
-                            a.lse[static_cast<long>(h) * b.N + row] =
-                                l[nb][c] == 0.f ? -INFINITY : (m[nb][c] + log2f(l[nb][c])) * kLn2;
-                    } else {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + VB * g);
-#pragma unroll
-                        for (int q = 0; q < VB / 4; ++q) dst[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
-                        if (g == 0) p.part_ml[static_cast<long>(slot) * MR + r] = make_float2(m[nb][c], l[nb][c]);
-                    }
-                }
-            if (lane == 0 && x.t0 > 0 && x.t1 == x.tiles)
-                p.joins[blockIdx.x] = Join{line.owner(x.first), x.row0, rows, x.q0, x.hk};
+                for (int j = 0; j < NJ; ++j)
+                    mine[(nb * NJ + j) * 32 + lane] = make_float4(o[nb][j][0], o[nb][j][1], o[nb][j][2], o[nb][j][3]);
         }
+        arrive(&sm.meet);
+        if (!await(&sm.meet, met)) return;
+        met ^= 1;
+        if (warp < 2) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                if (warp == 0 && g == 0) {
+                    sm.row[8 * nb + 2 * t] = make_float2(m[nb][0], l[nb][0]);
+                    sm.row[8 * nb + 2 * t + 1] = make_float2(m[nb][1], l[nb][1]);
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float4 y = mine[(nb * NJ + j) * 32 + lane];
+                    y.x += o[nb][j][0];
+                    y.y += o[nb][j][1];
+                    y.z += o[nb][j][2];
+                    y.w += o[nb][j][3];
+                    mine[(nb * NJ + j) * 32 + lane] = y;
+                }
+            }
+            arrive(&sm.o_full);
+        }
+        arrive(&sm.piece_empty[i % PIECES]);
     }
 }
 
@@ -851,7 +949,8 @@ ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, 
     // Row tiles of 8, 16 or 32, the smallest that holds a sequence's rows on average: fewer row tiles read
     // the cache less often, smaller ones leave fewer idle rows.
     const long per_seq = (static_cast<long>(b.N) * p.G + b.S - 1) / b.S;
-    const int NB = per_seq <= 8 ? 1 : per_seq <= 16 ? 2 : 4;
+    // (f32 rows of 128 columns stop at 16: pairs of q and O of 32 would leave no second stage.)
+    const int NB = per_seq <= 8 ? 1 : per_seq <= 16 || (a.dtype == KATTN_F32 && D == 128) ? 2 : 4;
     const int MR = 8 * NB, ctas = 2 * num_sms;
     const bool join = (static_cast<long>(b.max_pages) << p.page_shift) > TK;  // else no item has two tiles
     ProjStatus st;
@@ -875,8 +974,11 @@ ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, 
     }
     if (st.ok()) {
         auto pick = [&](auto d, auto fmt, auto nb, auto split) {
-            return launch<decltype(d)::value, decltype(fmt)::value, decltype(nb)::value, decltype(split)::value>(
-                p, ctas, join, s, launches);
+            if constexpr (decltype(split)::value && decltype(d)::value == 128 && decltype(nb)::value == 4)
+                return cudaErrorInvalidValue;
+            else
+                return launch<decltype(d)::value, decltype(fmt)::value, decltype(nb)::value, decltype(split)::value>(
+                    p, ctas, join, s, launches);
         };
         auto by_split = [&](auto d, auto fmt, auto nb) {
             return a.dtype == KATTN_F32 ? pick(d, fmt, nb, std::true_type{}) : pick(d, fmt, nb, std::false_type{});

@@ -736,7 +736,7 @@ class KVCache:
                 raise ValueError(f"{name} is on another device than k")
         self.k, self.v, self.k_scale, self.v_scale, self.format = k, v, k_scale, v_scale, int(fmt)
         self.n_pages, self.n_kv_head, self.page_size, self.d = k.shape
-        self.device = k.device
+        self.device_index = k.get_device()
         self._table = KVCacheTable(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.n_pages,
                                    self.page_size, self.n_kv_head, self.d, self.format)
         self._ref = ctypes.byref(self._table)
@@ -752,72 +752,101 @@ class KVCache:
                    torch.zeros(shape[:3], device=device), torch.zeros(shape[:3], device=device), fmt)
 
 
-_dtype_codes = None
+# The checks below run on every call of a decoding loop: they compare device
+# indices and type singletons rather than build objects, and pass plain
+# integers to ctypes.
+_codes = {}  # torch type -> KATTN_F32 / KATTN_BF16 / KATTN_F16
+
+
+def _types():
+    import torch
+
+    _codes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    return _codes
 
 
 def _dtype_code(t, name):
     """KATTN_F32 / KATTN_BF16 / KATTN_F16."""
-    global _dtype_codes
-    if _dtype_codes is None:
-        import torch
-
-        _dtype_codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    code = _dtype_codes.get(t.dtype)
+    code = (_codes or _types()).get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16")
     return code
 
 
-def _packed(t, name, like, cols):
-    """(pointer, row stride) of a [rows, cols] view of `like`'s type and device."""
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name} must be {like.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, not {like.device}")
-    if t.dim() != 2 or t.shape[1] != cols:
-        raise ValueError(f"{name} must be [rows, {cols}]")
-    if t.stride(1) != 1:
+def _on(ctx, t, name):
+    """The index of the tensor's device, which has to be the context's."""
+    index = t.get_device()  # -1: not on a GPU
+    if index != ctx.device:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    return index
+
+
+def _packed(t, name, dtype, device, rows, cols):
+    """Row stride of a [rows, cols] view (rows < 0: any number) of this type on this device."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on device {device}")
+    if t.dim() != 2 or t.shape[1] != cols or 0 <= rows != t.shape[0]:
+        raise ValueError(f"{name} must be [{rows if rows >= 0 else 'rows'}, {cols}]")
+    ld, inner = t.stride()
+    if inner != 1:
         raise ValueError(f"{name} must have unit inner stride")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), cols))
+    return ld if ld > cols else cols if t.shape[0] < 2 else ld
 
 
 def _ints(t, name, n, device):
-    if t.dtype != _int32() or not t.is_contiguous() or t.device != device or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on {device}")
+    if t.dtype is not _int32() or t.get_device() != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements on device {device}")
     return t.data_ptr()
 
 
+_kinds = {}
+
+
 def _int32():
+    return _kinds.get(32) or _kind(32)
+
+
+def _int64():
+    return _kinds.get(64) or _kind(64)
+
+
+def _kind(bits):
     import torch
-    return torch.int32
+
+    _kinds.update({32: torch.int32, 64: torch.int64, "f32": torch.float32,
+                   "stream": torch._C._cuda_getCurrentRawStream})
+    return _kinds[bits]
 
 
-def _on(ctx, t, name):
-    """The tensor's device, which has to be the context's."""
-    device = t.device
-    if device.type != "cuda" or device.index != ctx.device:
-        raise ValueError(f"{name} is on {device}, the context on cuda:{ctx.device}")
-    return device
+def _raw_stream(stream, device):
+    """The cudaStream_t of `stream`, or of torch's current one on the device."""
+    if stream is not None:
+        return stream.cuda_stream
+    return (_kinds.get("stream") or _kind("stream"))(device)
 
 
 def _sums(lse, n_head, n, device):
-    if lse.dtype != _f32() or not lse.is_contiguous() or tuple(lse.shape) != (n_head, n) or lse.device != device:
-        raise ValueError(f"lse must be a contiguous float32 tensor of shape ({n_head}, {n}) on {device}")
+    if (lse.dtype is not (_kinds.get("f32") or _kind("f32")) or lse.get_device() != device or lse.dim() != 2
+            or lse.shape[0] != n_head or lse.shape[1] != n or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 tensor of shape ({n_head}, {n}) on device {device}")
     return lse.data_ptr()
 
 
 def _pages(cache, cu, kv_len, table, device):
-    """The arguments that place a batch in the cache."""
-    if cache.device != device:
-        raise ValueError(f"the cache is on {cache.device}, not {device}")
+    """The arguments that place a batch in the cache, and its sequences."""
+    if cache.device_index != device:
+        raise ValueError(f"the cache is on device {cache.device_index}, not {device}")
     S = kv_len.shape[0]
-    if table.dtype != _int32() or table.device != device or table.dim() != 2 or table.shape[0] != S:
-        raise ValueError(f"table must be an int32 [{S}, pages] tensor on {device}")
+    if table.dtype is not _int32() or table.get_device() != device or table.dim() != 2 or table.shape[0] != S:
+        raise ValueError(f"table must be an int32 [{S}, pages] tensor on device {device}")
     pages = table.shape[1]
-    if pages > 1 and table.stride(1) != 1:
+    ld, inner = table.stride()
+    if pages > 1 and inner != 1:
         raise ValueError("table must have unit inner stride")
     return (_ints(cu, "cu", S + 1, device), _ints(kv_len, "kv_len", S, device), table.data_ptr(),
-            max(table.stride(0), pages), pages), S
+            ld if ld > pages else pages, pages), S
 
 
 def fwd_packed(ctx: Context, q, k, v, o, lse, cu_q, cu_k, n_head: int, n_kv_head: int | None = None,
@@ -830,24 +859,25 @@ def fwd_packed(ctx: Context, q, k, v, o, lse, cu_q, cu_k, n_head: int, n_kv_head
     if n_head <= 0 or kv <= 0:
         raise ValueError("head counts must be positive")
     device = _on(ctx, q, "q")
+    code = _dtype_code(q, "q")
+    dtype = q.dtype
     N, C = q.shape
     d = C // n_head
-    dtype = _dtype_code(q, "q")
-    pq, ldq = _packed(q, "q", q, n_head * d)
-    pk, ldk = _packed(k, "k", q, kv * d)
-    pv, ldv = _packed(v, "v", q, kv * d)
-    po, ldo = _packed(o, "o", q, C)
-    if k.shape[0] != v.shape[0] or o.shape[0] != N:
-        raise ValueError("q and o, k and v must have the same rows")
-    if ldk != ldv:
+    ldq = _packed(q, "q", dtype, device, N, n_head * d)
+    ldk = _packed(k, "k", dtype, device, -1, kv * d)
+    Nk = k.shape[0]
+    if _packed(v, "v", dtype, device, Nk, kv * d) != ldk:
         raise ValueError("k, v must share one row stride")
+    ldo = _packed(o, "o", dtype, device, N, C)
     S = cu_q.shape[0] - 1
-    st = lib().kattn_fwd_packed(ctx.handle, dtype, pq, ldq, pk, pv, ldk, po, ldo, _sums(lse, n_head, N, device),
-                                _ints(cu_q, "cu_q", S + 1, device), _ints(cu_k, "cu_k", S + 1, device), S, N,
-                                k.shape[0], n_head, kv, d, 1.0 / math.sqrt(d) if scale is None else scale,
-                                1 if causal else 0, _stream_ptr(stream, device))
-    _check(st, "kattn_fwd_packed")
-    return last_launch_count()
+    L = lib()
+    st = L.kattn_fwd_packed(ctx._h, code, q.data_ptr(), ldq, k.data_ptr(), v.data_ptr(), ldk, o.data_ptr(), ldo,
+                            _sums(lse, n_head, N, device), _ints(cu_q, "cu_q", S + 1, device),
+                            _ints(cu_k, "cu_k", S + 1, device), S, N, Nk, n_head, kv, d,
+                            d ** -0.5 if scale is None else scale, 1 if causal else 0, _raw_stream(stream, device))
+    if st:
+        _check(st, "kattn_fwd_packed")
+    return L.kattn_last_launch_count()
 
 
 def cache_append(ctx: Context, cache: KVCache, k, v, cu, kv_len, table, stream=None) -> int:
@@ -865,17 +895,19 @@ def cache_read(ctx: Context, cache: KVCache, k, v, cu, kv_len, table, stream=Non
 
 def _cache_rows(what, ctx, cache, k, v, cu, kv_len, table, stream):
     device = _on(ctx, k, "k")
-    dtype = _dtype_code(k, "k")
+    code = _dtype_code(k, "k")
     cols = cache.n_kv_head * cache.d
-    pk, ldk = _packed(k, "k", k, cols)
-    pv, ldv = _packed(v, "v", k, cols)
-    if ldk != ldv or k.shape[0] != v.shape[0]:
-        raise ValueError("k, v must share their rows and one row stride")
+    N = k.shape[0]
+    ld = _packed(k, "k", k.dtype, device, N, cols)
+    if _packed(v, "v", k.dtype, device, N, cols) != ld:
+        raise ValueError("k, v must share one row stride")
     where, S = _pages(cache, cu, kv_len, table, device)
-    st = getattr(lib(), what)(ctx.handle, cache._ref, dtype, pk, pv, ldk, *where, S, k.shape[0],
-                              _stream_ptr(stream, device))
-    _check(st, what)
-    return last_launch_count()
+    L = lib()
+    st = getattr(L, what)(ctx._h, cache._ref, code, k.data_ptr(), v.data_ptr(), ld, *where, S, N,
+                          _raw_stream(stream, device))
+    if st:
+        _check(st, what)
+    return L.kattn_last_launch_count()
 
 
 def fwd_cached(ctx: Context, cache: KVCache, q, o, lse, cu, kv_len, table, n_head: int, tree=None,
@@ -885,26 +917,21 @@ def fwd_cached(ctx: Context, cache: KVCache, q, o, lse, cu, kv_len, table, n_hea
     gives, as bits, the drafted tokens that each row sees (None: those up to its own).
     lse [n_head, N].  Returns kernels launched."""
     device = _on(ctx, q, "q")
-    N = q.shape[0]
-    d = cache.d
-    dtype = _dtype_code(q, "q")
-    pq, ldq = _packed(q, "q", q, n_head * d)
-    po, ldo = _packed(o, "o", q, n_head * d)
-    if o.shape[0] != N:
-        raise ValueError("q and o must have the same rows")
+    code = _dtype_code(q, "q")
+    N, d = q.shape[0], cache.d
+    ldq = _packed(q, "q", q.dtype, device, N, n_head * d)
+    ldo = _packed(o, "o", q.dtype, device, N, n_head * d)
     where, S = _pages(cache, cu, kv_len, table, device)
     bits = None
     if tree is not None:
-        if tree.dtype != _int64() or not tree.is_contiguous() or tuple(tree.shape) != (N,) or tree.device != device:
-            raise ValueError(f"tree must be a contiguous int64 tensor of {N} elements on {device}")
+        if (tree.dtype is not _int64() or tree.get_device() != device or tree.dim() != 1 or tree.shape[0] != N
+                or not tree.is_contiguous()):
+            raise ValueError(f"tree must be a contiguous int64 tensor of {N} elements on device {device}")
         bits = tree.data_ptr()
-    st = lib().kattn_fwd_cached(ctx.handle, cache._ref, dtype, pq, ldq, po, ldo, _sums(lse, n_head, N, device),
-                                *where, bits, S, N, n_head, 1.0 / math.sqrt(d) if scale is None else scale,
-                                _stream_ptr(stream, device))
-    _check(st, "kattn_fwd_cached")
-    return last_launch_count()
-
-
-def _int64():
-    import torch
-    return torch.int64
+    L = lib()
+    st = L.kattn_fwd_cached(ctx._h, cache._ref, code, q.data_ptr(), ldq, o.data_ptr(), ldo,
+                            _sums(lse, n_head, N, device), *where, bits, S, N, n_head,
+                            d ** -0.5 if scale is None else scale, _raw_stream(stream, device))
+    if st:
+        _check(st, "kattn_fwd_cached")
+    return L.kattn_last_launch_count()

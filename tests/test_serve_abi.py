@@ -121,16 +121,20 @@ def test_binding_refusals():
         kerr_attn.fwd_packed(Fake, x, x, x, x, torch.zeros(1, 4), i, i, 0)
     with pytest.raises(TypeError):
         kerr_attn._dtype_code(torch.zeros(1, dtype=torch.float64), "q")
-    with pytest.raises(TypeError):
-        kerr_attn._packed(x.half(), "k", x, 64)
-    with pytest.raises(ValueError):
-        kerr_attn._packed(x, "k", x, 32)
-    with pytest.raises(ValueError):
-        kerr_attn._packed(x.T, "k", x, 4)
-    with pytest.raises(ValueError):
-        kerr_attn._ints(i.long(), "cu", 2, i.device)
-    with pytest.raises(ValueError):
-        kerr_attn._ints(i, "cu", 3, i.device)
+    for bad, kind in ((lambda: kerr_attn._packed(x.half(), "k", x.dtype, -1, 4, 64), TypeError),
+                      (lambda: kerr_attn._packed(x, "k", x.dtype, 0, 4, 64), ValueError),   # another device
+                      (lambda: kerr_attn._packed(x, "k", x.dtype, -1, 4, 32), ValueError),  # columns
+                      (lambda: kerr_attn._packed(x, "k", x.dtype, -1, 5, 64), ValueError),  # rows
+                      (lambda: kerr_attn._packed(x.T, "k", x.dtype, -1, 64, 4), ValueError),
+                      (lambda: kerr_attn._ints(i.long(), "cu", 2, -1), ValueError),
+                      (lambda: kerr_attn._ints(i, "cu", 3, -1), ValueError),
+                      (lambda: kerr_attn._ints(i, "cu", 2, 0), ValueError),
+                      (lambda: kerr_attn._sums(torch.zeros(4, 1), 1, 4, -1), ValueError)):
+        with pytest.raises(kind):
+            bad()
+    assert kerr_attn._packed(x, "k", x.dtype, -1, -1, 64) == 64
+    assert kerr_attn._packed(x[:, :32], "k", x.dtype, -1, 4, 32) == 64
+    assert kerr_attn._packed(x[:1, :32], "k", x.dtype, -1, 1, 32) == 64
 
 
 def test_plain_forms_agree():
