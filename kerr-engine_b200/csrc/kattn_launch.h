@@ -185,7 +185,7 @@ struct PackedArgs {
     int* status = nullptr;
     unsigned long long wait_ns = 1000000000ull;
 };
-ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaStream_t s, int* launches);
+ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
 
 // A batch's place in a paged cache.
 struct CacheArgs {

@@ -12,10 +12,13 @@
 // a work item is 256 of them: two tiles of 128, which read the same K and V
 // tiles.  A group of few tokens then still fills its tile.
 //
+// Work.  With many items to a CTA, each takes whole ones, longest first.  A
+// small problem's items are one line of key tiles cut into equal parts, one a CTA
+// (few long sequences then still fill the GPU); packed_join adds the parts of cut items.
+//
 // Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
-// one thread a row.  8-11: Q into shared memory (and, for f32, K and V, split into bf16
-// hi and lo).  12: issues every MMA.  13: TMA of K and V (16-bit types).  14:
-// finds the CTA's items.  While one row tile is in its softmax, the tensor core
+// one thread a row.  8-11: Q into shared memory (and, for f32, K and V split in place into bf16
+// hi and lo).  12: issues every MMA.  13: TMA of K and V.  14: walks the CTA's work.  While one row tile is in its softmax, the tensor core
 // works on the other: O += P V of the tile before, then S = Q K^T of the next.
 //
 // TMEM.  S of each row tile (BN columns; P is packed over it) and O of each
@@ -61,7 +64,8 @@ struct Cfg {
     static constexpr int ROW = D == 32 ? 64 : 128;           // bytes of a row of a swizzled block
     static constexpr int BLOCKS = D == 128 ? 2 : 1;          // 64-column blocks (32 at D = 32) of a row
     static constexpr int Q_BLOCK = BM * ROW, Q_PART = BLOCKS * Q_BLOCK, Q_BYTES = PARTS * Q_PART;
-    static constexpr int KV_BLOCK = BN * ROW, KV_PART = BLOCKS * KV_BLOCK, KV_BYTES = PARTS * KV_PART;
+    // A K or V tile: per block its rows (f32: as the copy lands them, then hi rows and lo rows in their place).
+    static constexpr int KV_PART = BN * ROW, KV_BLOCK = PARTS * KV_PART, KV_BYTES = BLOCKS * KV_BLOCK;
     static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
     static constexpr bool BF16 = !std::is_same_v<T, __half>;
@@ -75,26 +79,59 @@ struct Cfg {
     __host__ __device__ static constexpr uint32_t col_p(int s) { return SPLIT ? 32 * (s >> 1) + 8 * (s & 1) : 8 * s; }
 };
 
+// A work item, or, where the line of work was cut, a part of one: the key
+// tiles from the shift-th key on.
 struct Item {
-    int q0, nq, k0, nk;  // the sequence's rows and keys
-    int hk;              // key head
-    int r0;              // first row of the item among the sequence's nq * G
-    int n0, n1;          // key tiles of each row tile
+    int q0, nq, nk;   // the sequence's first row, its rows and keys
+    int k0, shift;    // the first key row here, and how many of the sequence lie before it
+    int hk;           // key head
+    int r0;           // first row of the item among the sequence's nq * G
+    int n0, n1;       // key tiles of each row tile
+    int slot;         // where a part's sums go; -1: the item is whole
     int valid;
     __device__ __forceinline__ int n(int t) const { return t ? n1 : n0; }
+};
+
+// An item whose parts packed_join adds.
+struct Join {
+    int first_cta;  // holds the item's first part; -1: this CTA ends no item that others began
+    int q0, nq, hk, r0;
+};
+
+// A border of the line of work: before tile `tile` of item `item` (numbered
+// through the key heads).
+struct Border {
+    int item, tile;
+};
+
+// Small problems: the items of one key head and their running cost, while a
+// CTA looks for its part of the line.
+constexpr int PLAN = 1024;
+struct Plan {
+    int2 seq[PLAN];   // rows and keys of each sequence
+    int item0[PLAN];  // its first item
+    int cost[PLAN];   // running cost of the items
+    int warp_sum[N_THREADS / 32];
 };
 
 template <class T, int D>
 struct Smem {
     using C = Cfg<T, D>;
     alignas(1024) uint8_t q[2][C::Q_BYTES];
-    alignas(1024) uint8_t kv[C::STAGES][C::KV_BYTES];
+    union {
+        alignas(1024) uint8_t kv[C::STAGES][C::KV_BYTES];
+        Plan plan;  // before the first copy
+    };
+    uint64_t raw_full[C::STAGES];  // f32: the copy has landed
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_ready[2], o_full[2];
     uint64_t kv_full[C::STAGES], kv_empty[C::STAGES];
     uint64_t item_full[ITEMS], item_empty[ITEMS];
     uint64_t tail, drain;
     Item items[ITEMS];
+    Border from, to;  // the CTA's part of the line
+    int first_cta;    // of the item that `from` cuts
+    int head_items;   // items of a key head
     uint32_t tmem_slot;
 };
 
@@ -104,12 +141,23 @@ struct Params {
     int G;     // query heads of a key head
     float c;   // |scale| log2(e)
     int flip;  // scale < 0: the rows of Q are negated
+    int line;  // a small problem
+    float4* part_o;   // [2 * CTAs][D / 4][256 rows]: a CTA's part that began before it (0) or begins in it (1)
+    float2* part_ml;  // [2 * CTAs][256 rows]: row maxima (times c) and sums
+    Join* joins;      // [CTAs]
 };
 
 // ---------------------------------------------------------------- items
-// A row's keys: the first `seen` of its sequence.
-__device__ __forceinline__ int row_seen(const Item& it, int token, int causal) {
-    return causal ? min(max(token + it.nk - it.nq + 1, 0), it.nk) : it.nk;
+// A row's keys: the first of its sequence, so many.
+__device__ __forceinline__ int row_seen(int nq, int nk, int token, int causal) {
+    return causal ? min(max(token + nk - nq + 1, 0), nk) : nk;
+}
+
+// Key tiles of the row tile of rows r .. r + 127 of a sequence's nq * G.
+template <int BN>
+__device__ __forceinline__ int key_tiles(int nq, int nk, int G, int causal, int r) {
+    const int last = min(nq * G, r + BM) - 1;
+    return last < r ? 0 : (row_seen(nq, nk, last / G, causal) + BN - 1) / BN;
 }
 
 // How many of a sequence's items take at least c key tiles.
@@ -198,10 +246,183 @@ struct ItemFinder {
             }
             rank -= __shfl_sync(0xffffffffu, sum, 31);
         }
-        const int rows = it.nq * G;
-        const int end0 = min(rows, it.r0 + BM) - 1, end1 = min(rows, it.r0 + 2 * BM) - 1;  // last rows of the tiles
-        it.n0 = (row_seen(it, end0 / G, a.causal) + BN - 1) / BN;
-        it.n1 = end1 < it.r0 + BM ? 0 : (row_seen(it, end1 / G, a.causal) + BN - 1) / BN;
+        it.shift = 0;
+        it.slot = -1;
+        it.n0 = key_tiles<BN>(it.nq, it.nk, G, a.causal, it.r0);
+        it.n1 = key_tiles<BN>(it.nq, it.nk, G, a.causal, it.r0 + BM);
+        return it;
+    }
+};
+
+// Small problems: all items are one line of key tiles, ITEM_COST more for
+// each (its rows, its output), cut into equal parts of at least MIN_PART.  A
+// border moves to an item's edge that is near.
+constexpr int ITEM_COST = 4, MIN_PART = 6;
+constexpr long LINE_ITEMS = 6;  // items to a CTA below which a problem is small
+
+template <int BN>
+__device__ __forceinline__ int item_cost(int2 seq, int G, int causal, int item) {
+    const int r = item * ITEM_ROWS;
+    return ITEM_COST + max(key_tiles<BN>(seq.x, seq.y, G, causal, r), key_tiles<BN>(seq.x, seq.y, G, causal, r + BM));
+}
+
+// Running sums of x0, x1 (elements 2 tid and 2 tid + 1) over the block's threads.
+__device__ __forceinline__ void block_scan(int& x0, int& x1, int* warp_sum, int tid) {
+    const int lane = tid & 31;
+    const int own = x0 + x1;
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+    }
+    if (lane == 31) warp_sum[tid >> 5] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < (tid >> 5); ++w) before += warp_sum[w];
+    __syncthreads();
+    x0 += before + sum - own;
+    x1 += x0;
+}
+
+// The last element of the ascending v[0 .. n-1] that is <= x (v[0] is).
+__device__ __forceinline__ int last_up_to(const int* v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// The CTA's part of the line, by the whole block: fills from, to, first_cta and head_items.
+template <int BN, class S>
+__device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
+    const PackedArgs& a = p.a;
+    Plan& pl = sm.plan;
+    int x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int s = 2 * tid + u;
+        x[u] = 0;
+        if (s < a.S) {
+            const int2 q = seq_rows(a.cu_q, s, a.Nq), k = seq_rows(a.cu_k, s, a.Nk);
+            pl.seq[s] = make_int2(q.y - q.x, k.y - k.x);
+            x[u] = ((q.y - q.x) * p.G + ITEM_ROWS - 1) / ITEM_ROWS;
+        }
+    }
+    const int own0 = x[0], own1 = x[1];
+    block_scan(x[0], x[1], pl.warp_sum, tid);
+    if (2 * tid < a.S) pl.item0[2 * tid] = x[0] - own0;
+    if (2 * tid + 1 < a.S) pl.item0[2 * tid + 1] = x[1] - own1;
+    if (tid == N_THREADS - 1) sm.head_items = x[1];
+    __syncthreads();
+    const int items = sm.head_items;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int e = 2 * tid + u;
+        x[u] = 0;
+        if (e < items) {
+            const int s = last_up_to(pl.item0, a.S, e);
+            x[u] = item_cost<BN>(pl.seq[s], p.G, a.causal, e - pl.item0[s]);
+        }
+    }
+    block_scan(x[0], x[1], pl.warp_sum, tid);
+    if (2 * tid < items) pl.cost[2 * tid] = x[0];
+    if (2 * tid + 1 < items) pl.cost[2 * tid + 1] = x[1];
+    __syncthreads();
+    if (tid == 0) {
+        const int head = items > 0 ? pl.cost[items - 1] : 0;
+        const long total = static_cast<long>(head) * a.Hkv;
+        const long ctas = min(static_cast<long>(gridDim.x), max(total / MIN_PART, 1L));
+        auto border = [&](long b) -> Border {
+            if (b >= ctas || total == 0) return Border{items * a.Hkv, 0};
+            const long at = b * total / ctas;
+            const int hk = static_cast<int>(at / head), in = static_cast<int>(at % head);
+            int lo = -1, hi = items - 1;  // the first item whose running cost passes `in`
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (pl.cost[mid] > in) hi = mid;
+                else lo = mid;
+            }
+            const int start = hi > 0 ? pl.cost[hi - 1] : 0, cost = pl.cost[hi] - start, off = in - start;
+            const int near = static_cast<int>(total / ctas / 8) + ITEM_COST;
+            if (off <= near) return Border{hk * items + hi, 0};
+            if (cost - off <= near) return Border{hk * items + hi + 1, 0};
+            return Border{hk * items + hi, off - ITEM_COST};
+        };
+        const long b = blockIdx.x;
+        const Border from = border(b);
+        sm.from = from;
+        sm.to = border(b + 1);
+        long first = b;
+        if (from.tile > 0) {
+            Border y;
+            do y = border(--first);
+            while (y.item == from.item && y.tile > 0);
+        }
+        sm.first_cta = static_cast<int>(first);
+    }
+    fence_async_smem();  // the plan's place is the copies' next
+    __syncthreads();
+}
+
+// Walks the CTA's part of the line; a whole warp, every lane alike.
+template <int BN>
+struct LineWalker {
+    const Params& p;
+    Border at, to;
+    int cta, first_cta, head_items;
+    int hk, s, i, tiles;  // key head, sequence, item of the sequence and of how many
+    int2 q, k;
+
+    __device__ __forceinline__ void load(int seq) {
+        s = seq;
+        q = seq_rows(p.a.cu_q, s, p.a.Nq);
+        k = seq_rows(p.a.cu_k, s, p.a.Nk);
+        tiles = ((q.y - q.x) * p.G + ITEM_ROWS - 1) / ITEM_ROWS;
+    }
+    __device__ __forceinline__ void start() {
+        if (at.item >= head_items * p.a.Hkv) return;
+        hk = at.item / head_items;
+        i = at.item % head_items;
+        load(0);
+        while (i >= tiles) {
+            i -= tiles;
+            load(s + 1);
+        }
+    }
+    __device__ __forceinline__ Item next() {
+        Item it;
+        it.valid = at.item < to.item || (at.item == to.item && at.tile < to.tile);
+        if (!it.valid) return it;
+        it.q0 = q.x;
+        it.nq = q.y - q.x;
+        it.nk = k.y - k.x;
+        it.hk = hk;
+        it.r0 = i * ITEM_ROWS;
+        const int n0 = key_tiles<BN>(it.nq, it.nk, p.G, p.a.causal, it.r0);
+        const int n1 = key_tiles<BN>(it.nq, it.nk, p.G, p.a.causal, it.r0 + BM);
+        const int all = max(n0, n1), t0 = at.tile, t1 = at.item == to.item ? to.tile : all;
+        it.shift = t0 * BN;
+        it.k0 = k.x + it.shift;
+        it.n0 = max(min(n0, t1) - t0, 0);
+        it.n1 = max(min(n1, t1) - t0, 0);
+        it.slot = t0 == 0 && t1 == all ? -1 : 2 * cta + (t0 == 0 ? 1 : 0);
+        if (t0 > 0 && t1 == all && (threadIdx.x & 31) == 0)
+            p.joins[cta] = Join{first_cta, it.q0, it.nq, it.hk, it.r0};
+        at = Border{at.item + 1, 0};
+        if (++i == tiles && (at.item < to.item || (at.item == to.item && to.tile > 0))) {
+            i = 0;
+            int y = s + 1;
+            if (at.item % head_items == 0) {
+                ++hk;
+                y = 0;
+            }
+            load(y);
+            while (tiles == 0) load(s + 1);
+        }
         return it;
     }
 };
@@ -268,32 +489,39 @@ __device__ __forceinline__ void load_q(const Params& p, const Item& it, int t, u
     }
 }
 
-// A tile of BN f32 rows (K or V) held in registers by the 128 loader threads
-// between its loads and its conversion; rows past the sequence's are zeros.
-template <int D, int BN>
+// A K or V tile of f32 rows as the copy lands it (blocks of 64 columns, 32 at
+// D = 32, row-major) -> the same bytes as swizzled bf16 hi rows and lo rows, by the
+// 128 loader threads: all read before any writes.  Rows from `rows` on, the next
+// sequence's, become zeros: their weights are zero, and zero times an infinity is not.
+template <int D>
 struct F32Tile {
-    static constexpr int CH = D / 8, N = BN * CH / 128;
-    float4 x[N][2];
-    __device__ __forceinline__ void load(const float* base, long ld, int rows, int tid) {
+    using C = Cfg<float, D>;
+    static constexpr int W = D < 64 ? D : 64, Q4 = W / 4;           // columns and float4 of a block's row
+    static constexpr int N = C::BN * Q4 / 128;                      // float4 of a block for a thread
+    float4 x[C::BLOCKS][N];
+    __device__ __forceinline__ void read(const uint8_t* tile, int rows, int tid) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int u = tid + i * 128, r = u / CH, ch = u % CH;
-            x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows) {
-                const float4* src = reinterpret_cast<const float4*>(base + r * ld + ch * 8);
-                x[i][0] = __ldg(src);
-                x[i][1] = __ldg(src + 1);
+        for (int b = 0; b < C::BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int f = tid + i * 128;
+                x[b][i] = reinterpret_cast<const float4*>(tile + b * C::KV_BLOCK)[f];
+                if (f / Q4 >= rows) x[b][i] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-        }
     }
-    template <int PART, int BLOCK>
-    __device__ __forceinline__ void store(uint8_t* dst, int tid) const {
+    __device__ __forceinline__ void write(uint8_t* tile, int tid) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int u = tid + i * 128, r = u / CH, ch = u % CH;
-            put8<float, D, PART, BLOCK>(dst, r, ch, *reinterpret_cast<const uint4*>(&x[i][0]),
-                                        *reinterpret_cast<const uint4*>(&x[i][1]));
-        }
+        for (int b = 0; b < C::BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int f = tid + i * 128, r = f / Q4, c4 = f % Q4;
+                uint2 h, l;
+                split2_x2(x[b][i].x, x[b][i].y, h.x, l.x);
+                split2_x2(x[b][i].z, x[b][i].w, h.y, l.y);
+                uint8_t* at = tile + b * C::KV_BLOCK + swizzled<float, D>(r, c4 >> 1) + (c4 & 1) * 8;
+                *reinterpret_cast<uint2*>(at) = h;
+                *reinterpret_cast<uint2*>(at + C::KV_PART) = l;
+            }
     }
 };
 
@@ -365,6 +593,28 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
     return fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7]));
 }
 
+// 32 columns of an output row, rounded once.
+template <class T>
+__device__ __forceinline__ void store32(T* out, const float (&o)[32]) {
+    uint4* dst = reinterpret_cast<uint4*>(out);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            dst[u] = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]), __float_as_uint(o[4 * u + 2]),
+                                __float_as_uint(o[4 * u + 3]));
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                w[x] = std::is_same_v<T, __half> ? pack_f16(o[8 * u + 2 * x], o[8 * u + 2 * x + 1])
+                                                 : pack_bf16(o[8 * u + 2 * x], o[8 * u + 2 * x + 1]);
+            dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- kernel
 template <class T, int D>
 __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant__ Params p) {
@@ -389,11 +639,12 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         }
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&sm.kv_full[i], C::SPLIT ? 128 : 1);
+            mbar_init(&sm.raw_full[i], 1);
             mbar_init(&sm.kv_empty[i], 1);
         }
         for (int i = 0; i < ITEMS; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_empty[i], C::SPLIT ? 13 : 14);  // softmax 8, loader 4, MMA, TMA
+            mbar_init(&sm.item_empty[i], 14);  // softmax 8, loader 4, MMA, TMA
         }
         mbar_init(&sm.tail, 1);
         mbar_init(&sm.drain, 1);
@@ -403,6 +654,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
     __syncthreads();
     tc_fence_after();
     pdl_wait();
+    if (p.line) plan_line<BN>(sm, p, tid);
     const uint32_t tm = sm.tmem_slot;
     const uint64_t limit = p.a.wait_ns;
     bool failed = false;
@@ -435,7 +687,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             const int row = it.r0 + t * BM + rl;
             const bool mine = row < it.nq * p.G;
             const int token = row / p.G;
-            const int seen = mine ? row_seen(it, token, p.a.causal) : 0;
+            const int seen = mine ? row_seen(it.nq, it.nk, token, p.a.causal) - it.shift : 0;
             const int n = it.n(t);
             float mu = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j, ++g) {
@@ -508,15 +760,6 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 mbar_arrive(&sm.p_ready[t]);
             }
             if (failed) break;
-            // Output: normalised, rounded once; rows that saw nothing are zeros.
-            const float inv = seen > 0 ? 1.f / l : 0.f;
-            T* out = nullptr;
-            if (mine) {
-                const int h = it.hk * p.G + row % p.G;
-                out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D;
-                p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
-                    seen > 0 ? (mu * p.c + log2f(l)) * kLn2 : -INFINITY;
-            }
             if (n > 0) {
                 if (!mbar_wait_warp(&sm.o_full[t], done & 1, limit)) {
                     failed = true;
@@ -524,6 +767,33 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 }
                 ++done;
                 tc_fence_after();
+            }
+            if (it.slot >= 0) {
+                // A part: its sums as they are, columns in fours so that neighbouring rows' stores touch.
+                const int r = t * BM + rl;
+                float4* dst = p.part_o + static_cast<long>(it.slot) * (D / 4) * ITEM_ROWS + r;
+                p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
+                if (n > 0) {
+#pragma unroll
+                    for (int q = 0; q < D / 32; ++q) {
+                        float o[32];
+                        tmem_ld32(to + 32 * q, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            dst[(8 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    }
+                }
+                continue;
+            }
+            // Output: normalised, rounded once; rows that saw nothing are zeros.
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            T* out = nullptr;
+            if (mine) {
+                const int h = it.hk * p.G + row % p.G;
+                out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D;
+                p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
+                    l == 0.f ? -INFINITY : (mu * p.c + log2f(l)) * kLn2;
             }
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
@@ -534,24 +804,8 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 }
                 if (mine) {
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = seen > 0 ? o[u] * inv : 0.f;
-                    uint4* dst = reinterpret_cast<uint4*>(out + 32 * q);
-                    if constexpr (C::SPLIT) {
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            dst[u] = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]),
-                                                __float_as_uint(o[4 * u + 2]), __float_as_uint(o[4 * u + 3]));
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                w[x] = C::BF16 ? pack_bf16(o[8 * u + 2 * x], o[8 * u + 2 * x + 1])
-                                               : pack_f16(o[8 * u + 2 * x], o[8 * u + 2 * x + 1]);
-                            dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
+                    for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
+                    store32<T>(out + 32 * q, o);
                 }
             }
         }
@@ -581,18 +835,18 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 mbar_arrive(&sm.q_full[t]);
             }
             if constexpr (C::SPLIT) {
-                // K_0, V_0, K_1, ...: a tile's loads are in flight while its stage is waited for.
+                // K_0, V_0, K_1, ...: each converted in place once it has landed.
                 const int n = max(it.n0, it.n1);
                 for (int x = 0; x < 2 * n && !failed; ++x, ++kv) {
-                    const int j = x >> 1, st = kv % C::STAGES, turn = kv / C::STAGES;
-                    F32Tile<D, BN> tile;
-                    tile.load(static_cast<const float*>(x & 1 ? p.a.v : p.a.k) + static_cast<long>(it.k0 + j * BN) * p.a.ld_kv + it.hk * D, p.a.ld_kv,
-                              it.nk - j * BN, lt);
-                    if (turn > 0 && !mbar_wait_warp(&sm.kv_empty[st], (turn - 1) & 1, limit)) {
+                    const int st = kv % C::STAGES;
+                    const bool ok = mbar_wait(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
+                    F32Tile<D> tile;
+                    tile.read(sm.kv[st], it.nk - it.shift - (x >> 1) * BN, lt);
+                    if (named_sync_or(1, 128, !ok || failed)) {
                         failed = true;
                         break;
                     }
-                    tile.template store<C::KV_PART, C::KV_BLOCK>(sm.kv[st], lt);
+                    tile.write(sm.kv[st], lt);
                     fence_async_smem();
                     mbar_arrive(&sm.kv_full[st]);
                 }
@@ -661,7 +915,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 mbar_wait(&sm.drain, 0, 10000000ull);
             }
             __syncwarp();
-        } else if (warp == TMA_WARP && !C::SPLIT) {
+        } else if (warp == TMA_WARP) {
             // -------------------------------------------------------- K / V copies
             if (lane == 0 && p.a.Nk > 0) {
                 prefetch_tensormap(&p.tk);
@@ -685,9 +939,9 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     const CUtensorMap* map = x & 1 ? &p.tv : &p.tk;
                     // A V tile past the sequence's end holds rows of the next one, whose weights are zero: those
                     // rows are cleared, as zero times an infinity or a NaN there would not be zero.
-                    const int rows = it.nk - j * BN;
-                    const bool tail = (x & 1) && rows < BN;
-                    uint64_t* bar = tail ? &sm.tail : &sm.kv_full[st];
+                    const int rows = it.nk - it.shift - j * BN;
+                    const bool tail = !C::SPLIT && (x & 1) && rows < BN;
+                    uint64_t* bar = C::SPLIT ? &sm.raw_full[st] : tail ? &sm.tail : &sm.kv_full[st];
                     if (lane == 0) {
                         mbar_arrive_expect_tx(bar, C::KV_BYTES);
 #pragma unroll
@@ -711,16 +965,20 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             if (failed) {
                 // Copies still landing complete before the shared memory is released.
                 for (int x = max(0, kv - C::STAGES); x < kv; ++x)
-                    mbar_wait(&sm.kv_full[x % C::STAGES], (x / C::STAGES) & 1, 10000000ull);
+                    mbar_wait(C::SPLIT ? &sm.raw_full[x % C::STAGES] : &sm.kv_full[x % C::STAGES], (x / C::STAGES) & 1,
+                              10000000ull);
                 if (tails > 0) mbar_wait(&sm.tail, (tails - 1) & 1, 10000000ull);
             }
         } else if (warp == ITEM_WARP) {
             // -------------------------------------------------------- items
-            ItemFinder<BN> find{p.a, p.G, lane, 0, 0};
-            find.start();
             const int ctas = gridDim.x, b = blockIdx.x;
+            if (p.line && lane == 0) p.joins[b].first_cta = -1;
+            ItemFinder<BN> find{p.a, p.G, lane, 0, 0};
+            LineWalker<BN> walk{p, sm.from, sm.to, b, sm.first_cta, sm.head_items};
+            if (p.line) walk.start();
+            else find.start();
             for (int i = 0;; ++i) {
-                const Item it = find.find(i * ctas + (i & 1 ? ctas - 1 - b : b));
+                const Item it = p.line ? walk.next() : find.find(i * ctas + (i & 1 ? ctas - 1 - b : b));
                 const int slot = i % ITEMS;
                 if (i >= ITEMS && !mbar_wait_warp(&sm.item_empty[slot], (i / ITEMS - 1) & 1, limit)) {
                     failed = true;
@@ -741,57 +999,129 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
     if (warp == MMA_WARP) tmem_dealloc(tm, TMEM_COLS);
 }
 
+// Adds the parts of the items that borders cut: block (c, y) the rows 32y ..
+// 32y + 31, one lane each, of the item that CTA c ended.  The parts lie in the CTAs
+// from the join's first to c, one each, and are added in that order; the
+// block's four warps share the columns.
 template <class T, int D>
-cudaError_t launch(const PackedArgs& a, int num_sms, cudaStream_t stream) {
+__global__ void __launch_bounds__(128) packed_join(const __grid_constant__ Params p) {
+    constexpr int E = D / 4;  // columns of a warp
+    pdl_enter();
+    const int c = blockIdx.x, r = 32 * blockIdx.y + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    const Join j = p.joins[c];
+    const int row = j.r0 + r;
+    if (j.first_cta < 0 || row >= j.nq * p.G) return;
+    float acc[E], big = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int q = j.first_cta; q <= c; ++q) {
+        const long slot = 2L * q + (q == j.first_cta ? 1 : 0);
+        const float2 ml = p.part_ml[slot * ITEM_ROWS + r];
+        if (ml.y == 0.f) continue;  // the row saw none of the part's keys
+        const float top = fmaxf(big, ml.x);
+        const float keep = ex2(big - top), mine = ex2(ml.x - top);
+        big = top;
+        l = fmaf(l, keep, ml.y * mine);
+        const float4* src = p.part_o + (slot * (D / 4) + w * (E / 4)) * ITEM_ROWS + r;
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) {
+            const float4 v = src[e * ITEM_ROWS];
+            acc[4 * e] = fmaf(acc[4 * e], keep, v.x * mine);
+            acc[4 * e + 1] = fmaf(acc[4 * e + 1], keep, v.y * mine);
+            acc[4 * e + 2] = fmaf(acc[4 * e + 2], keep, v.z * mine);
+            acc[4 * e + 3] = fmaf(acc[4 * e + 3], keep, v.w * mine);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int h = j.hk * p.G + row % p.G;
+    const long at = j.q0 + row / p.G;
+    T* out = static_cast<T*>(p.a.o) + at * p.a.ld_o + h * D + w * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 16 / static_cast<int>(sizeof(T))) {
+        Vec16<T> y;
+#pragma unroll
+        for (int i = 0; i < Vec16<T>::N; ++i) y.x[i] = from_f32<T>(acc[e + i] * inv);
+        *reinterpret_cast<uint4*>(out + e) = y.raw;
+    }
+    if (w == 0) p.a.lse[static_cast<long>(h) * p.a.Nq + at] = l == 0.f ? -INFINITY : (big + log2f(l)) * kLn2;
+}
+
+template <class T, int D>
+ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t stream, int* launches) {
     using C = Cfg<T, D>;
+    ProjStatus st;
+    st.what = "packed forward launch";
     Params p{};
     p.a = a;
     p.G = a.H / a.Hkv;
     // A scale of zero weighs every key alike; kept positive so that a masked score stays -inf.
     p.c = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
     p.flip = a.scale < 0.f;
-    if constexpr (!C::SPLIT) {
-        if (a.Nk > 0) {
+    if (a.Nk > 0) {
+        const long cols = static_cast<long>(a.Hkv) * D;
+        const int box = D == 32 ? 32 : 64;
+        bool ok;
+        if constexpr (C::SPLIT) {
+            ok = encode_2d(&p.tk, static_cast<const float*>(a.k), cols, a.Nk, a.ld_kv, box, C::BN) &&
+                 encode_2d(&p.tv, static_cast<const float*>(a.v), cols, a.Nk, a.ld_kv, box, C::BN);
+        } else {
             const CUtensorMapSwizzle sw = D == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-            const long cols = static_cast<long>(a.Hkv) * D;
-            const int box = D == 32 ? 32 : 64;
-            if (!encode_2d_bf16(&p.tk, static_cast<const uint16_t*>(a.k), cols, a.Nk, a.ld_kv, box, C::BN, sw) ||
-                !encode_2d_bf16(&p.tv, static_cast<const uint16_t*>(a.v), cols, a.Nk, a.ld_kv, box, C::BN, sw))
-                return cudaErrorInvalidValue;
+            ok = encode_2d_bf16(&p.tk, static_cast<const uint16_t*>(a.k), cols, a.Nk, a.ld_kv, box, C::BN, sw) &&
+                 encode_2d_bf16(&p.tv, static_cast<const uint16_t*>(a.v), cols, a.Nk, a.ld_kv, box, C::BN, sw);
+        }
+        if (!ok) {
+            st.cuda = cudaErrorInvalidValue;
+            return st;
         }
     }
     auto kernel = packed_fwd<T, D>;
     constexpr size_t smem = sizeof(Smem<T, D>) + 1024;
     static_assert(smem <= SMEM_MAX, "shared memory");
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
+    st.cuda = cudaGetDevice(&dev);
+    if (!st.ok()) return st;
     static std::atomic<uint64_t> attr_done{0};  // one bit per device
     const uint64_t bit = 1ull << (dev & 63);
     if (!(attr_done.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
+        st.cuda = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (!st.ok()) return st;
         attr_done.fetch_or(bit);
     }
-    // No more items than this: each sequence ends at most one item that is not full.
-    const long items = (static_cast<long>(a.Nq) * p.G / ITEM_ROWS + a.S) * a.Hkv;
-    return launch_pdl(kernel, dim3(static_cast<unsigned>(items < num_sms ? items : num_sms)), dim3(N_THREADS), smem,
-                      stream, p);
+    // Each sequence ends at most one item that is not full.
+    const long head_items = static_cast<long>(a.Nq) * p.G / ITEM_ROWS + a.S;
+    p.line = head_items <= PLAN && head_items * a.Hkv < LINE_ITEMS * num_sms;
+    const int ctas = p.line || head_items * a.Hkv > num_sms ? num_sms : static_cast<int>(head_items * a.Hkv);
+    char* ws = nullptr;
+    const size_t o_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS * D, ml_bytes = sizeof(float2) * 2 * ctas * ITEM_ROWS;
+    if (p.line) {
+        st.cuda = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), o_bytes + ml_bytes + sizeof(Join) * ctas, pool, stream);
+        if (!st.ok()) return st;
+        p.part_o = reinterpret_cast<float4*>(ws);
+        p.part_ml = reinterpret_cast<float2*>(ws + o_bytes);
+        p.joins = reinterpret_cast<Join*>(ws + o_bytes + ml_bytes);
+    }
+    st.cuda = launch_pdl(kernel, dim3(ctas), dim3(N_THREADS), smem, stream, p);
+    if (st.ok()) ++*launches;
+    if (p.line) {
+        if (st.ok()) {
+            st.cuda = launch_pdl(packed_join<T, D>, dim3(ctas, ITEM_ROWS / 32), dim3(128), 0, stream, p);
+            if (st.ok()) ++*launches;
+        }
+        const cudaError_t freed = cudaFreeAsync(ws, stream);
+        if (st.ok()) st.cuda = freed;
+    }
+    return st;
 }
 
 }  // namespace
 
-ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaStream_t s, int* launches) {
-    ProjStatus st;
-    st.what = "packed forward launch";
+ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches) {
     auto pick = [&](auto f32, auto bf16, auto f16) {
-        return (a.dtype == KATTN_F32 ? f32 : a.dtype == KATTN_BF16 ? bf16 : f16)(a, num_sms, s);
+        return (a.dtype == KATTN_F32 ? f32 : a.dtype == KATTN_BF16 ? bf16 : f16)(a, num_sms, pool, s, launches);
     };
-    st.cuda = a.d == 32   ? pick(launch<float, 32>, launch<__nv_bfloat16, 32>, launch<__half, 32>)
-              : a.d == 64 ? pick(launch<float, 64>, launch<__nv_bfloat16, 64>, launch<__half, 64>)
-                          : pick(launch<float, 128>, launch<__nv_bfloat16, 128>, launch<__half, 128>);
-    if (st.ok()) ++*launches;
-    return st;
+    return a.d == 32   ? pick(launch<float, 32>, launch<__nv_bfloat16, 32>, launch<__half, 32>)
+           : a.d == 64 ? pick(launch<float, 64>, launch<__nv_bfloat16, 64>, launch<__half, 64>)
+                       : pick(launch<float, 128>, launch<__nv_bfloat16, 128>, launch<__half, 128>);
 }
 
 }  // namespace kattn

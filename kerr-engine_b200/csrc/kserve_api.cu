@@ -140,7 +140,7 @@ int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const 
                               scale, causal, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed)};
     int launches = 0;
     const kattn::ProjStatus st =
-        kattn::packed_forward(a, ctx->num_sms, static_cast<cudaStream_t>(stream), &launches);
+        kattn::packed_forward(a, ctx->num_sms, ctx->pool, static_cast<cudaStream_t>(stream), &launches);
     return result(st, launches);
 }
 
