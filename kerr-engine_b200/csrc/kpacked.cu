@@ -16,9 +16,9 @@
 // small problem's items are one line of key tiles cut into equal parts, one a CTA
 // (few long sequences then still fill the GPU); packed_join adds the parts of cut items.
 //
-// Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
-// one thread a row.  8-11: Q into shared memory (and, for f32, K and V split in place into bf16
-// hi and lo).  12: issues every MMA.  13: TMA of K and V.  14: walks the CTA's work.  While one row tile is in its softmax, the tensor core
+// Warps (24).  0-7 and 8-15: the softmax of the first and the second row tile,
+// two threads a row, half of the tile's keys each.  16-19: Q into shared memory (and, for f32, K and V split
+// in place into bf16 hi and lo).  20: issues every MMA.  21: TMA of K and V.  22: walks the CTA's work.  While one row tile is in its softmax, the tensor core
 // works on the other: O += P V of the tile before, then S = Q K^T of the next.
 //
 // TMEM.  S of each row tile (BN columns; P is packed over it) and O of each
@@ -48,10 +48,9 @@ using namespace sm100;
 
 constexpr int BM = 128;          // rows of a row tile
 constexpr int ITEM_ROWS = 2 * BM;
-constexpr int N_THREADS = 512;
-constexpr int LOAD_WARP = 8, MMA_WARP = 12, TMA_WARP = 13, ITEM_WARP = 14;
+constexpr int N_THREADS = 768, LAUNCH_REGS = 80;  // 65536 / 768, in eights
+constexpr int LOAD_WARP = 16, MMA_WARP = 20, TMA_WARP = 21, ITEM_WARP = 22;
 constexpr int ITEMS = 4;         // item ring
-constexpr int HELD = 64;         // columns of a row of S held in registers
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr size_t SMEM_MAX = 227 * 1024;
@@ -66,12 +65,13 @@ struct Cfg {
     static constexpr int Q_BLOCK = BM * ROW, Q_PART = BLOCKS * Q_BLOCK, Q_BYTES = PARTS * Q_PART;
     // A K or V tile: per block its rows (f32: as the copy lands them, then hi rows and lo rows in their place).
     static constexpr int KV_PART = BN * ROW, KV_BLOCK = PARTS * KV_PART, KV_BYTES = BLOCKS * KV_BLOCK;
-    static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - 2 * Q_BYTES) / KV_BYTES);
+    static constexpr int TURNS = SPLIT && D == 128 ? 1 : 2;  // buffers of the exchange between a row's threads
+    static constexpr int FIT = static_cast<int>((SMEM_MAX - 1024 - TURNS * 2048 - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
     static constexpr bool BF16 = !std::is_same_v<T, __half>;
-    // Registers of a softmax, loader and service thread (512 threads of 128 at launch).
-    static constexpr int R_SOFT = SPLIT ? 168 : 184, R_LOAD = SPLIT ? 112 : 80, R_SERV = 64;
-    static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 512, "register split");
+    // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
+    static constexpr int R_SOFT = SPLIT ? 88 : 96, R_LOAD = SPLIT ? 88 : 56, R_SERV = 40;
+    static_assert(4 * R_SOFT + R_LOAD + R_SERV <= 6 * LAUNCH_REGS, "register split");
     __host__ __device__ static constexpr uint32_t col_s(int t) { return t * BN; }
     __host__ __device__ static constexpr uint32_t col_o(int t) { return 2 * BN + t * D; }
     static_assert(2 * BN + 2 * D <= 512, "TMEM columns");
@@ -132,6 +132,7 @@ struct Smem {
     Border from, to;  // the CTA's part of the line
     int first_cta;    // of the item that `from` cuts
     int head_items;   // items of a key head
+    float half[C::TURNS][2][2][BM];  // what the two threads of a row exchange, by turn, row tile and half
     uint32_t tmem_slot;
 };
 
@@ -568,19 +569,6 @@ __device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool fi
 }
 
 // ---------------------------------------------------------------- softmax
-// N columns of this thread's row of S; those from `lim` on are masked where
-// `masked` (the same for the warp).
-template <int N>
-__device__ __forceinline__ void load_scores(uint32_t at, float (&s)[N], bool masked, int lim) {
-#pragma unroll
-    for (int q = 0; q < N / 32; ++q) tmem_ld32(at + 32 * q, reinterpret_cast<float(&)[32]>(s[32 * q]));
-    tmem_wait_ld();
-    if (masked) {
-#pragma unroll
-        for (int q = 0; q < N; ++q) s[q] = q < lim ? s[q] : -INFINITY;
-    }
-}
-
 template <int N>
 __device__ __forceinline__ float row_max(const float (&s)[N]) {
     float mx[8];
@@ -593,18 +581,18 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
     return fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7]));
 }
 
-// 32 columns of an output row, rounded once.
+// 16 columns of an output row, rounded once.
 template <class T>
-__device__ __forceinline__ void store32(T* out, const float (&o)[32]) {
+__device__ __forceinline__ void store16(T* out, const float (&o)[16]) {
     uint4* dst = reinterpret_cast<uint4*>(out);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < 4; ++u)
             dst[u] = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]), __float_as_uint(o[4 * u + 2]),
                                 __float_as_uint(o[4 * u + 3]));
     } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
@@ -620,9 +608,13 @@ template <class T, int D>
 __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant__ Params p) {
     using C = Cfg<T, D>;
     constexpr int BN = C::BN;
-    extern __shared__ uint8_t smem_raw[];
-    Smem<T, D>& sm = *reinterpret_cast<Smem<T, D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem<T, D>& sm = *reinterpret_cast<Smem<T, D>*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem_raw) % 1024 != 0) {  // swizzled tiles need it; there is no room to align by hand
+        if (tid == 0) atomicOr(p.a.status, 1);
+        return;
+    }
 
     pdl_launch();
     if (warp == MMA_WARP) {
@@ -634,7 +626,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             mbar_init(&sm.q_full[i], 128);
             mbar_init(&sm.q_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_ready[i], 128);
+            mbar_init(&sm.p_ready[i], 8);
             mbar_init(&sm.o_full[i], 1);
         }
         for (int i = 0; i < C::STAGES; ++i) {
@@ -644,7 +636,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         }
         for (int i = 0; i < ITEMS; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_empty[i], 14);  // softmax 8, loader 4, MMA, TMA
+            mbar_init(&sm.item_empty[i], 22);  // softmax 16, loader 4, MMA, TMA
         }
         mbar_init(&sm.tail, 1);
         mbar_init(&sm.drain, 1);
@@ -671,52 +663,74 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
 
     if (warp < LOAD_WARP) {
         // ------------------------------------------------------------ softmax
-        regs_inc<C::R_SOFT>();
-        const int t = warp >> 2;
+        regs_to<C::R_SOFT, LAUNCH_REGS>();
+        constexpr int W = BN / 2, DW = D / 2;  // this thread's share of the keys and of O's columns
+        const int t = warp >> 3, hf = (warp >> 2) & 1;
         const int rl = (warp & 3) * 32 + lane;
+        const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the row's two warps
         const uint32_t lb = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = lb + tm + C::col_s(t), to = lb + tm + C::col_o(t);
-        int g = 0, done = 0;  // tiles and items of this row tile so far
-        Item it;
+        const uint32_t ts = lb + tm + C::col_s(t), to = lb + tm + C::col_o(t) + hf * DW;
+        int g = 0, done = 0, turn = 0;  // tiles and items of this row tile so far, exchanges
+        bool bad = false;
+        // The other thread's value; true: a wait of one of the two warps ran out (both learn it here, and leave).
+        auto exchange = [&](float mine, float& other) {
+            sm.half[turn][t][hf][rl] = mine;
+            tc_fence_before();  // this thread's reads of S come before the other's P
+            const bool stop = named_sync_or(pair, 64, bad);
+            tc_fence_after();
+            other = sm.half[turn][t][hf ^ 1][rl];
+            if constexpr (C::TURNS == 2) turn ^= 1;
+            else named_sync(pair, 64);
+            return stop;
+        };
         for (int i = 0;; ++i) {
-            if (!get_item(i, it)) {
+            const Item& it = sm.items[i % ITEMS];  // stays in shared memory: registers are the scores'
+            bad |= !mbar_wait_warp(&sm.item_full[i % ITEMS], (i / ITEMS) & 1, limit);
+            if (named_sync_or(pair, 64, bad)) {
                 failed = true;
                 break;
             }
             if (!it.valid) break;
-            const int row = it.r0 + t * BM + rl;
-            const bool mine = row < it.nq * p.G;
-            const int token = row / p.G;
-            const int seen = mine ? row_seen(it.nq, it.nk, token, p.a.causal) - it.shift : 0;
+            auto release = [&] {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.item_empty[i % ITEMS]);
+            };
+            int seen;
+            {
+                const int row = it.r0 + t * BM + rl;
+                seen = row < it.nq * p.G ? row_seen(it.nq, it.nk, row / p.G, p.a.causal) - it.shift : 0;
+            }
             const int n = it.n(t);
             float mu = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j, ++g) {
-                if (!mbar_wait_warp(&sm.s_full[t], g & 1, limit)) {
+                bad |= !mbar_wait_warp(&sm.s_full[t], g & 1, limit);
+                tc_fence_after();
+                float s[W];
+#pragma unroll
+                for (int q = 0; q < W / 32; ++q)
+                    tmem_ld32(ts + hf * W + 32 * q, reinterpret_cast<float(&)[32]>(s[32 * q]));
+                tmem_wait_ld();
+                const int lim = seen - j * BN - hf * W;  // visible columns of these
+                if (__any_sync(0xffffffffu, lim < W)) {
+#pragma unroll
+                    for (int q = 0; q < W; ++q) s[q] = q < lim ? s[q] : -INFINITY;
+                }
+                float m = row_max<W>(s), other;
+                if (exchange(m, other)) {
                     failed = true;
                     break;
                 }
-                tc_fence_after();
-                // The row's maximum.  Half of a 128-column row is held in registers from here to its
-                // weights, the other half is read twice: the whole row does not fit beside the rest.
-                const int lim = seen - j * BN;  // visible columns of the tile
-                const bool masked = __any_sync(0xffffffffu, lim < BN);
-                float s[HELD], m = -INFINITY;
-#pragma unroll
-                for (int q = BN / HELD - 1; q >= 0; --q) {
-                    load_scores<HELD>(ts + HELD * q, s, masked, lim - HELD * q);
-                    m = fmaxf(m, row_max<HELD>(s));
-                }
+                m = fmaxf(m, other);
                 if (j == 0) {
                     mu = m;
                 } else {
                     const bool raise = (m - mu) * p.c > RESCALE_LOG2 || (mu == -INFINITY && m > mu);
                     if (__any_sync(0xffffffffu, raise)) {
-                        const float to_mu = raise ? m : mu;
                         const float f = raise ? ex2((mu - m) * p.c) : 1.f;
-                        mu = to_mu;
+                        mu = raise ? m : mu;
                         l *= f;
 #pragma unroll 1
-                        for (int q = 0; q < D / 16; ++q) {  // few columns at a time: the row of S is held meanwhile
+                        for (int q = 0; q < DW / 16; ++q) {  // few columns at a time: the scores are held meanwhile
                             float o[16];
                             uint32_t r[16];
                             tmem_ld16(to + 16 * q, o);
@@ -730,16 +744,14 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 const float off = mu == -INFINITY ? 0.f : -mu * p.c;
                 const uint64_t c2 = f2_pack(p.c, p.c), off2 = f2_pack(off, off);
                 uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
+                // P over S: every column has been read (the exchange above is behind both threads' reads).
 #pragma unroll
-                for (int q = 0; q < BN / 32; ++q) {
-                    if (q > 0 && q % (HELD / 32) == 0)
-                        load_scores<HELD>(ts + 32 * q, s, masked, lim - 32 * q);
-                    uint32_t hi[16], lo[16];
+                for (int q = 0; q < W / 16; ++q) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        const int v = (32 * q) % HELD + 2 * u;
+                    for (int u = 0; u < 8; ++u) {
                         float x, y;
-                        f2_unpack(f2_fma(f2_pack(s[v], s[v + 1]), c2, off2), x, y);
+                        f2_unpack(f2_fma(f2_pack(s[16 * q + 2 * u], s[16 * q + 2 * u + 1]), c2, off2), x, y);
                         x = ex2(x);
                         y = ex2(y);
                         if (u & 1) sum1 = f2_add(sum1, f2_pack(x, y));
@@ -748,70 +760,76 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         else if constexpr (C::BF16) hi[u] = pack_bf16(x, y);
                         else hi[u] = pack_f16(x, y);
                     }
-                    // Over columns that have been read for the last time: this chunk's own or an earlier one's.
-                    tmem_st16(ts + C::col_p(2 * q), hi);
-                    if constexpr (C::SPLIT) tmem_st16(ts + C::col_p(2 * q) + 16, lo);
+                    const uint32_t at = ts + C::col_p(hf * (W / 16) + q);
+                    tmem_st8(at, hi);
+                    if constexpr (C::SPLIT) tmem_st8(at + 16, lo);
                 }
                 float a0, a1;
                 f2_unpack(f2_add(sum0, sum1), a0, a1);
                 l += a0 + a1;
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&sm.p_ready[t]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_ready[t]);
             }
             if (failed) break;
+            float l2;
+            if (exchange(l, l2)) {
+                failed = true;
+                break;
+            }
+            l = hf ? l2 + l : l + l2;  // in the same order in both
             if (n > 0) {
-                if (!mbar_wait_warp(&sm.o_full[t], done & 1, limit)) {
-                    failed = true;
-                    break;
-                }
+                bad |= !mbar_wait_warp(&sm.o_full[t], done & 1, limit);
                 ++done;
                 tc_fence_after();
             }
             if (it.slot >= 0) {
                 // A part: its sums as they are, columns in fours so that neighbouring rows' stores touch.
                 const int r = t * BM + rl;
-                float4* dst = p.part_o + static_cast<long>(it.slot) * (D / 4) * ITEM_ROWS + r;
-                p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
+                float4* dst = p.part_o + (static_cast<long>(it.slot) * (D / 4) + hf * (DW / 4)) * ITEM_ROWS + r;
+                if (hf == 0) p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
                 if (n > 0) {
 #pragma unroll
-                    for (int q = 0; q < D / 32; ++q) {
-                        float o[32];
-                        tmem_ld32(to + 32 * q, o);
+                    for (int q = 0; q < DW / 16; ++q) {
+                        float o[16];
+                        tmem_ld16(to + 16 * q, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            dst[(8 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        for (int u = 0; u < 4; ++u)
+                            dst[(4 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                     }
                 }
+                release();
                 continue;
             }
             // Output: normalised, rounded once; rows that saw nothing are zeros.
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            T* out = nullptr;
-            if (mine) {
-                const int h = it.hk * p.G + row % p.G;
-                out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D;
+            const int row = it.r0 + t * BM + rl;
+            const bool mine = row < it.nq * p.G;
+            const int token = row / p.G, h = it.hk * p.G + row % p.G;
+            T* out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D + hf * DW;
+            if (mine && hf == 0)
                 p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
                     l == 0.f ? -INFINITY : (mu * p.c + log2f(l)) * kLn2;
-            }
 #pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-                float o[32];
+            for (int q = 0; q < DW / 16; ++q) {
+                float o[16];
                 if (n > 0) {
-                    tmem_ld32(to + 32 * q, o);
+                    tmem_ld16(to + 16 * q, o);
                     tmem_wait_ld();
                 }
                 if (mine) {
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
-                    store32<T>(out + 32 * q, o);
+                    for (int u = 0; u < 16; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
+                    store16<T>(out + 16 * q, o);
                 }
             }
+            release();
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------ loaders
-        regs_dec<C::R_LOAD>();
+        regs_to<C::R_LOAD, LAUNCH_REGS>();
         const int lt = tid - 32 * LOAD_WARP;
         int used[2] = {0, 0}, kv = 0;
         Item it;
@@ -842,7 +860,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     const bool ok = mbar_wait(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
                     F32Tile<D> tile;
                     tile.read(sm.kv[st], it.nk - it.shift - (x >> 1) * BN, lt);
-                    if (named_sync_or(1, 128, !ok || failed)) {
+                    if (named_sync_or(9, 128, !ok || failed)) {
                         failed = true;
                         break;
                     }
@@ -853,7 +871,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             }
         }
     } else {
-        regs_dec<C::R_SERV>();
+        regs_to<C::R_SERV, LAUNCH_REGS>();
         if (warp == MMA_WARP) {
             // -------------------------------------------------------- MMA issuer
             int kv = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
@@ -1075,7 +1093,7 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
         }
     }
     auto kernel = packed_fwd<T, D>;
-    constexpr size_t smem = sizeof(Smem<T, D>) + 1024;
+    constexpr size_t smem = sizeof(Smem<T, D>);
     static_assert(smem <= SMEM_MAX, "shared memory");
     int dev = 0;
     st.cuda = cudaGetDevice(&dev);

@@ -351,6 +351,12 @@ template <int REGS>
 __device__ __forceinline__ void regs_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
+// From FROM, the launch's registers a thread, to REGS: dec above FROM, or inc below it, is not a legal instruction.
+template <int REGS, int FROM>
+__device__ __forceinline__ void regs_to() {
+    if constexpr (REGS > FROM) regs_inc<REGS>();
+    else if constexpr (REGS < FROM) regs_dec<REGS>();
+}
 
 // ---------------------------------------------------------------- 256-bit global access
 // 32 bytes of read-only global memory in one 256-bit load (sm_100); p must
