@@ -534,7 +534,7 @@ __device__ __forceinline__ uint64_t k_major(uint32_t addr) {
 
 // S_t = Q_t K^T of the K tile at `k`: 16 columns of d a step.
 template <class T, int D>
-__device__ __forceinline__ void issue_s(uint32_t tm, int t, uint32_t q, uint32_t k) {
+__device__ __forceinline__ void issue_s(uint32_t tm, int t, uint32_t q, uint32_t k, uint32_t elected) {
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, C::BN, 0, 0) : idesc_f16(BM, C::BN, 0, 0);
     const uint32_t out = tm + C::col_s(t);
@@ -542,17 +542,18 @@ __device__ __forceinline__ void issue_s(uint32_t tm, int t, uint32_t q, uint32_t
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
         const uint32_t qo = (s >> 2) * C::Q_BLOCK + (s & 3) * 32, ko = (s >> 2) * C::KV_BLOCK + (s & 3) * 32;
-        mma_ss(out, desc_add(qd, qo), desc_add(kd, ko), id, s > 0);
+        if (s == 0) mma_ss_elected<false>(out, qd, kd, id, elected);
+        else mma_ss_elected<true>(out, desc_add(qd, qo), desc_add(kd, ko), id, elected);
         if constexpr (C::SPLIT) {
-            mma_ss(out, desc_add(qd, qo), desc_add(kd, ko + C::KV_PART), id, 1);
-            mma_ss(out, desc_add(qd, qo + C::Q_PART), desc_add(kd, ko), id, 1);
+            mma_ss_elected<true>(out, desc_add(qd, qo), desc_add(kd, ko + C::KV_PART), id, elected);
+            mma_ss_elected<true>(out, desc_add(qd, qo + C::Q_PART), desc_add(kd, ko), id, elected);
         }
     }
 }
 
 // O_t (+)= P_t V of the V tile at `v`: 16 keys a step; P's hi (and lo) words over S_t.
 template <class T, int D>
-__device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool first) {
+__device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool first, uint32_t elected) {
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, D, 0, 1) : idesc_f16(BM, D, 0, 1);
     const uint32_t out = tm + C::col_o(t), ph = tm + C::col_s(t);
@@ -560,10 +561,10 @@ __device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool fi
 #pragma unroll
     for (int s = 0; s < C::BN / 16; ++s) {
         const uint32_t o = s * 16 * C::ROW, ps = ph + C::col_p(s);
-        mma_ts(out, ps, desc_add(vd, o), id, (first && s == 0) ? 0u : 1u);
+        mma_ts_elected(out, ps, desc_add(vd, o), id, s > 0 ? 1u : first ? 0u : 1u, elected);
         if constexpr (C::SPLIT) {
-            mma_ts(out, ps, desc_add(vd, o + C::KV_PART), id, 1);
-            mma_ts(out, ps + 16, desc_add(vd, o), id, 1);
+            mma_ts_elected(out, ps, desc_add(vd, o + C::KV_PART), id, 1, elected);
+            mma_ts_elected(out, ps + 16, desc_add(vd, o), id, 1, elected);
         }
     }
 }
@@ -874,64 +875,73 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         regs_to<C::R_SERV, LAUNCH_REGS>();
         if (warp == MMA_WARP) {
             // -------------------------------------------------------- MMA issuer
-            int kv = 0, q_used[2] = {0, 0}, p_used[2] = {0, 0};
-            Item it;
+            // The whole warp walks in step and one lane issues; counts come from reductions, whose results are
+            // uniform to the compiler too.
+            const uint32_t one = elect_one();
+            const uint32_t q0 = smem_u32(sm.q[0]), q1 = smem_u32(sm.q[1]), kv0 = smem_u32(sm.kv[0]);
+            int st = 0;          // ring: the next tile's stage, and its phase
+            uint32_t phase = 0;
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
             for (int i = 0; !failed; ++i) {
+                Item it;
                 if (!get_item(i, it)) {
                     failed = true;
                     break;
                 }
-                if (!it.valid) break;
-                const int n = max(it.n0, it.n1);
+                if (!__reduce_max_sync(0xffffffffu, it.valid)) break;
+                const int nt[2] = {__reduce_max_sync(0xffffffffu, it.n0), __reduce_max_sync(0xffffffffu, it.n1)};
+                const int n = max(nt[0], nt[1]);
                 if (n == 0) continue;
-                if (lane == 0) {
-                    auto full = [&](int x) { return mbar_wait(&sm.kv_full[x % C::STAGES], (x / C::STAGES) & 1, limit); };
-                    failed = !full(kv);
+                if (!mbar_wait_warp(&sm.kv_full[st], phase, limit)) {
+                    failed = true;
+                    break;
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (failed || nt[t] == 0) continue;
+                    failed = !mbar_wait_warp(&sm.q_full[t], q_phase[t], limit);
+                    if (failed) continue;
+                    q_phase[t] ^= 1;
+                    tc_fence_after();
+                    issue_s<T, D>(tm, t, t ? q1 : q0, kv0 + st * C::KV_BYTES, one);
+                    mma_commit_elected(&sm.s_full[t], one);
+                    if (nt[t] == 1) mma_commit_elected(&sm.q_empty[t], one);
+                }
+                mma_commit_elected(&sm.kv_empty[st], one);
+                if (++st == C::STAGES) st = 0, phase ^= 1;
+                for (int j = 0; j < n && !failed; ++j) {
+                    const bool next = j + 1 < n;
+                    const int ks = st + 1 == C::STAGES ? 0 : st + 1;  // the next K tile's stage
+                    const uint32_t k_phase = ks == 0 ? phase ^ 1 : phase;
+                    failed = !mbar_wait_warp(&sm.kv_full[st], phase, limit);
+                    if (next && !failed) failed = !mbar_wait_warp(&sm.kv_full[ks], k_phase, limit);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (failed || it.n(t) == 0) continue;
-                        failed = !mbar_wait(&sm.q_full[t], q_used[t]++ & 1, limit);
+                        if (failed || j >= nt[t]) continue;
+                        failed = !mbar_wait_warp(&sm.p_ready[t], p_phase[t], limit);
                         if (failed) continue;
+                        p_phase[t] ^= 1;
                         tc_fence_after();
-                        issue_s<T, D>(tm, t, smem_u32(sm.q[t]), smem_u32(sm.kv[kv % C::STAGES]));
-                        mma_commit(&sm.s_full[t]);
-                        if (it.n(t) == 1) mma_commit(&sm.q_empty[t]);
-                    }
-                    mma_commit(&sm.kv_empty[kv % C::STAGES]);
-                    ++kv;
-                    for (int j = 0; j < n && !failed; ++j) {
-                        const bool next = j + 1 < n;
-                        failed = !full(kv);
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (failed || j >= it.n(t)) continue;
-                            failed = !mbar_wait(&sm.p_ready[t], p_used[t]++ & 1, limit);
-                            if (failed) continue;
-                            tc_fence_after();
-                            issue_pv<T, D>(tm, t, smem_u32(sm.kv[kv % C::STAGES]), j == 0);
-                            if (j + 1 < it.n(t)) {
-                                failed = !full(kv + 1);
-                                if (failed) continue;
-                                tc_fence_after();
-                                issue_s<T, D>(tm, t, smem_u32(sm.q[t]), smem_u32(sm.kv[(kv + 1) % C::STAGES]));
-                                mma_commit(&sm.s_full[t]);
-                                if (j + 2 == it.n(t)) mma_commit(&sm.q_empty[t]);
-                            } else {
-                                mma_commit(&sm.o_full[t]);
-                            }
+                        issue_pv<T, D>(tm, t, kv0 + st * C::KV_BYTES, j == 0, one);
+                        if (j + 1 < nt[t]) {
+                            issue_s<T, D>(tm, t, t ? q1 : q0, kv0 + ks * C::KV_BYTES, one);
+                            mma_commit_elected(&sm.s_full[t], one);
+                            if (j + 2 == nt[t]) mma_commit_elected(&sm.q_empty[t], one);
+                        } else {
+                            mma_commit_elected(&sm.o_full[t], one);
                         }
-                        mma_commit(&sm.kv_empty[kv % C::STAGES]);
-                        if (next) mma_commit(&sm.kv_empty[(kv + 1) % C::STAGES]);
-                        kv += next ? 2 : 1;
+                    }
+                    mma_commit_elected(&sm.kv_empty[st], one);
+                    if (++st == C::STAGES) st = 0, phase ^= 1;
+                    if (next) {
+                        mma_commit_elected(&sm.kv_empty[st], one);
+                        if (++st == C::STAGES) st = 0, phase ^= 1;
                     }
                 }
-                failed = __any_sync(0xffffffffu, failed);
             }
-            if (lane == 0) {
-                // MMAs still in flight complete before the columns are freed.
-                mma_commit(&sm.drain);
-                mbar_wait(&sm.drain, 0, 10000000ull);
-            }
+            // MMAs still in flight complete before the columns are freed.
+            mma_commit_elected(&sm.drain, one);
+            mbar_wait(&sm.drain, 0, 10000000ull);
             __syncwarp();
         } else if (warp == TMA_WARP) {
             // -------------------------------------------------------- K / V copies
