@@ -16,13 +16,17 @@
 // small problem's items are one line of key tiles cut into equal parts, one a CTA
 // (few long sequences then still fill the GPU); packed_join adds the parts of cut items.
 //
-// Warps (24).  0-7 and 8-15: the softmax of the first and the second row tile,
-// two threads a row, half of the tile's keys each.  16-19: Q into shared memory (and, for f32, K and V split
-// in place into bf16 hi and lo).  20: issues every MMA.  21: TMA of K and V.  22: walks the CTA's work.  While one row tile is in its softmax, the tensor core
-// works on the other: O += P V of the tile before, then S = Q K^T of the next.
+// Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
+// one thread a row.  8-11: Q into shared memory (and, for f32, K and V split
+// in place into bf16 hi and lo).  12: issues every MMA.  13: TMA of K and V.  14: walks
+// the CTA's work.
 //
-// TMEM.  S of each row tile (BN columns; P is packed over it) and O of each
-// (D columns): 512 columns at BN = D = 128.
+// Steps of 128 keys (64 for f32 at D = 128).  While one row tile is in its softmax,
+// the tensor core works on the other: O += P V of its step, then S = Q K^T of its next.
+// P goes over the S it came from, 64 keys at a time, and each half's product starts when
+// it is written.  (Steps of 64 keys with two S buffers a tile were slower: an MMA
+// with both operands in shared memory costs the same at N = 64 as at 128, the rows of Q
+// being the larger read.)  TMEM: 2 x 128 columns of S and P, 2 x D of O, 512 at D = 128.
 //
 // Types.  16-bit operands enter the MMAs as they are and P is rounded to the type; f32
 // ones as bf16 pairs, hi*hi + hi*lo + lo*hi (about 2^-17 of a product, where one
@@ -32,6 +36,7 @@
 // tile's maximum passes it by more than 2^8 (then O and the sum are scaled): weights
 // stay below 2^8, which f16 holds, and O is almost never read back.
 #include <atomic>
+#include <climits>
 
 #include <cuda.h>
 
@@ -48,10 +53,12 @@ using namespace sm100;
 
 constexpr int BM = 128;          // rows of a row tile
 constexpr int ITEM_ROWS = 2 * BM;
-constexpr int N_THREADS = 768, LAUNCH_REGS = 80;  // 65536 / 768, in eights
-constexpr int LOAD_WARP = 16, MMA_WARP = 20, TMA_WARP = 21, ITEM_WARP = 22;
+constexpr int HALF = 64;         // keys whose weights are handed over at once
+constexpr int N_THREADS = 512, LAUNCH_REGS = 128;
+constexpr int LOAD_WARP = 8, MMA_WARP = 12, TMA_WARP = 13, ITEM_WARP = 14;
 constexpr int ITEMS = 4;         // item ring
 constexpr float RESCALE_LOG2 = 8.f;
+constexpr int POLY = 1;          // of 8 pairs of weights by the FMA units (16-bit types)
 constexpr uint32_t TMEM_COLS = 512;
 constexpr size_t SMEM_MAX = 227 * 1024;
 
@@ -59,34 +66,34 @@ template <class T, int D>
 struct Cfg {
     static constexpr bool SPLIT = sizeof(T) == 4;            // operands as bf16 hi / lo pairs
     static constexpr int PARTS = SPLIT ? 2 : 1;
-    static constexpr int BN = SPLIT && D == 128 ? 64 : 128;  // keys of a tile (64: Q's pairs leave less room)
+    static constexpr int BN = SPLIT && D == 128 ? 64 : 128;  // keys of a step (64: Q's pairs leave less room)
+    static constexpr int HALVES = BN / HALF;
     static constexpr int ROW = D == 32 ? 64 : 128;           // bytes of a row of a swizzled block
     static constexpr int BLOCKS = D == 128 ? 2 : 1;          // 64-column blocks (32 at D = 32) of a row
     static constexpr int Q_BLOCK = BM * ROW, Q_PART = BLOCKS * Q_BLOCK, Q_BYTES = PARTS * Q_PART;
     // A K or V tile: per block its rows (f32: as the copy lands them, then hi rows and lo rows in their place).
     static constexpr int KV_PART = BN * ROW, KV_BLOCK = PARTS * KV_PART, KV_BYTES = BLOCKS * KV_BLOCK;
-    static constexpr int TURNS = SPLIT && D == 128 ? 1 : 2;  // buffers of the exchange between a row's threads
-    static constexpr int FIT = static_cast<int>((SMEM_MAX - 1024 - TURNS * 2048 - 2 * Q_BYTES) / KV_BYTES);
+    static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
     static constexpr bool BF16 = !std::is_same_v<T, __half>;
     // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
-    static constexpr int R_SOFT = SPLIT ? 88 : 96, R_LOAD = SPLIT ? 88 : 56, R_SERV = 40;
-    static_assert(4 * R_SOFT + R_LOAD + R_SERV <= 6 * LAUNCH_REGS, "register split");
+    static constexpr int R_SOFT = SPLIT ? 184 : 200, R_LOAD = SPLIT ? 96 : 64, R_SERV = 48;
+    static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 4 * LAUNCH_REGS, "register split");
     __host__ __device__ static constexpr uint32_t col_s(int t) { return t * BN; }
     __host__ __device__ static constexpr uint32_t col_o(int t) { return 2 * BN + t * D; }
     static_assert(2 * BN + 2 * D <= 512, "TMEM columns");
-    // P's words of the 16 keys of step s, relative to S: packed, or, for pairs, the hi words of 32 keys and then the lo.
+    // P's words of the 16 keys of k-step s, relative to S: packed, or, for pairs, the hi words of 32 keys and then the lo.
     __host__ __device__ static constexpr uint32_t col_p(int s) { return SPLIT ? 32 * (s >> 1) + 8 * (s & 1) : 8 * s; }
 };
 
-// A work item, or, where the line of work was cut, a part of one: the key
-// tiles from the shift-th key on.
+// A work item, or, where the line of work was cut, a part of one: the steps
+// from the shift-th key on.
 struct Item {
     int q0, nq, nk;   // the sequence's first row, its rows and keys
     int k0, shift;    // the first key row here, and how many of the sequence lie before it
     int hk;           // key head
     int r0;           // first row of the item among the sequence's nq * G
-    int n0, n1;       // key tiles of each row tile
+    int n0, n1;       // steps of each row tile
     int slot;         // where a part's sums go; -1: the item is whole
     int valid;
     __device__ __forceinline__ int n(int t) const { return t ? n1 : n0; }
@@ -98,7 +105,7 @@ struct Join {
     int q0, nq, hk, r0;
 };
 
-// A border of the line of work: before tile `tile` of item `item` (numbered
+// A border of the line of work: before step `tile` of item `item` (numbered
 // through the key heads).
 struct Border {
     int item, tile;
@@ -124,7 +131,7 @@ struct Smem {
     };
     uint64_t raw_full[C::STAGES];  // f32: the copy has landed
     uint64_t q_full[2], q_empty[2];
-    uint64_t s_full[2], p_ready[2], o_full[2];
+    uint64_t s_full[2], p_ready[2][2], o_full[2];  // by row tile (and half)
     uint64_t kv_full[C::STAGES], kv_empty[C::STAGES];
     uint64_t item_full[ITEMS], item_empty[ITEMS];
     uint64_t tail, drain;
@@ -132,7 +139,7 @@ struct Smem {
     Border from, to;  // the CTA's part of the line
     int first_cta;    // of the item that `from` cuts
     int head_items;   // items of a key head
-    float half[C::TURNS][2][2][BM];  // what the two threads of a row exchange, by turn, row tile and half
+    int from_hk, from_seq, from_i;  // the item at `from`: key head, sequence, item of the sequence
     uint32_t tmem_slot;
 };
 
@@ -140,12 +147,15 @@ struct Params {
     CUtensorMap tk, tv;
     PackedArgs a;
     int G;     // query heads of a key head
+    uint32_t inv_g;  // 2^32 / G + 1
     float c;   // |scale| log2(e)
     int flip;  // scale < 0: the rows of Q are negated
     int line;  // a small problem
     float4* part_o;   // [2 * CTAs][D / 4][256 rows]: a CTA's part that began before it (0) or begins in it (1)
     float2* part_ml;  // [2 * CTAs][256 rows]: row maxima (times c) and sums
     Join* joins;      // [CTAs]
+    // x / G for x below 2^32 / G (the product is off by less than x G / 2^32).
+    __device__ __forceinline__ int div(int x) const { return G == 1 ? x : static_cast<int>(__umulhi(x, inv_g)); }
 };
 
 // ---------------------------------------------------------------- items
@@ -154,14 +164,14 @@ __device__ __forceinline__ int row_seen(int nq, int nk, int token, int causal) {
     return causal ? min(max(token + nk - nq + 1, 0), nk) : nk;
 }
 
-// Key tiles of the row tile of rows r .. r + 127 of a sequence's nq * G.
+// Steps of the row tile of rows r .. r + 127 of a sequence's nq * G.
 template <int BN>
 __device__ __forceinline__ int key_tiles(int nq, int nk, int G, int causal, int r) {
     const int last = min(nq * G, r + BM) - 1;
     return last < r ? 0 : (row_seen(nq, nk, last / G, causal) + BN - 1) / BN;
 }
 
-// How many of a sequence's items take at least c key tiles.
+// How many of a sequence's items take at least c steps.
 template <int BN>
 __device__ __forceinline__ int items_at_least(int nq, int nk, int G, int causal, int c) {
     const int tiles = (nq * G + ITEM_ROWS - 1) / ITEM_ROWS;
@@ -173,9 +183,9 @@ __device__ __forceinline__ int items_at_least(int nq, int nk, int G, int causal,
     return token >= nq ? 0 : tiles - token * G / ITEM_ROWS;
 }
 
-// Items in order of their key tiles, longest first, dealt to the CTAs in
+// Items in order of their steps, longest first, dealt to the CTAs in
 // snake order: item k is in round k / CTAs.  A warp finds the k-th without a list: the
-// count of items with at least c tiles is a sum over the sequences, and c
+// count of items with at least c steps is a sum over the sequences, and c
 // only falls as k grows.
 template <int BN>
 struct ItemFinder {
@@ -184,6 +194,7 @@ struct ItemFinder {
 
     __device__ __forceinline__ int count(int c) const {
         int n = 0;
+#pragma unroll 1
         for (int s = lane; s < a.S; s += 32) {
             const int2 q = seq_rows(a.cu_q, s, a.Nq), k = seq_rows(a.cu_k, s, a.Nk);
             n += items_at_least<BN>(q.y - q.x, k.y - k.x, G, a.causal, c);
@@ -192,6 +203,7 @@ struct ItemFinder {
     }
     __device__ __forceinline__ void start() {
         int nk = 0;
+#pragma unroll 1
         for (int s = lane; s < a.S; s += 32) {
             const int2 k = seq_rows(a.cu_k, s, a.Nk);
             nk = max(nk, k.y - k.x);
@@ -213,7 +225,8 @@ struct ItemFinder {
             }
             level = lo;
         }
-        int rank = k - count(level + 1);  // among the items of exactly `level` tiles
+        int rank = k - count(level + 1);  // among the items of exactly `level` steps
+#pragma unroll 1
         for (int s0 = 0; s0 < a.S; s0 += 32) {
             const int s = s0 + lane;
             int2 q = make_int2(0, 0), kk = make_int2(0, 0);
@@ -255,7 +268,7 @@ struct ItemFinder {
     }
 };
 
-// Small problems: all items are one line of key tiles, ITEM_COST more for
+// Small problems: all items are one line of steps, ITEM_COST more for
 // each (its rows, its output), cut into equal parts of at least MIN_PART.  A
 // border moves to an item's edge that is near.
 constexpr int ITEM_COST = 4, MIN_PART = 6;
@@ -279,8 +292,8 @@ __device__ __forceinline__ void block_scan(int& x0, int& x1, int* warp_sum, int 
     }
     if (lane == 31) warp_sum[tid >> 5] = sum;
     __syncthreads();
-    int before = 0;
-    for (int w = 0; w < (tid >> 5); ++w) before += warp_sum[w];
+    int before = lane < (tid >> 5) ? warp_sum[lane] : 0;
+    before = __reduce_add_sync(0xffffffffu, before);
     __syncthreads();
     x0 += before + sum - own;
     x1 += x0;
@@ -289,6 +302,7 @@ __device__ __forceinline__ void block_scan(int& x0, int& x1, int* warp_sum, int 
 // The last element of the ascending v[0 .. n-1] that is <= x (v[0] is).
 __device__ __forceinline__ int last_up_to(const int* v, int n, int x) {
     int lo = 0, hi = n;
+#pragma unroll 1
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (v[mid] <= x) lo = mid;
@@ -333,37 +347,42 @@ __device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
     if (2 * tid < items) pl.cost[2 * tid] = x[0];
     if (2 * tid + 1 < items) pl.cost[2 * tid + 1] = x[1];
     __syncthreads();
-    if (tid == 0) {
-        const int head = items > 0 ? pl.cost[items - 1] : 0;
-        const long total = static_cast<long>(head) * a.Hkv;
-        const long ctas = min(static_cast<long>(gridDim.x), max(total / MIN_PART, 1L));
-        auto border = [&](long b) -> Border {
+    if (tid < 2) {  // the CTA's first border and its last; 32 bits hold the line (checked at launch)
+        const int head = items > 0 ? pl.cost[items - 1] : 0, total = head * a.Hkv;
+        const int ctas = min(static_cast<int>(gridDim.x), max(total / MIN_PART, 1));
+        const int share = total / ctas, left = total % ctas, near = share / 8 + ITEM_COST;
+        auto border = [&](int b) -> Border {
             if (b >= ctas || total == 0) return Border{items * a.Hkv, 0};
-            const long at = b * total / ctas;
-            const int hk = static_cast<int>(at / head), in = static_cast<int>(at % head);
+            const int at = b * share + b * left / ctas;
+            const int hk = at / head, in = at - hk * head;
             int lo = -1, hi = items - 1;  // the first item whose running cost passes `in`
+#pragma unroll 1
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (pl.cost[mid] > in) hi = mid;
                 else lo = mid;
             }
             const int start = hi > 0 ? pl.cost[hi - 1] : 0, cost = pl.cost[hi] - start, off = in - start;
-            const int near = static_cast<int>(total / ctas / 8) + ITEM_COST;
             if (off <= near) return Border{hk * items + hi, 0};
             if (cost - off <= near) return Border{hk * items + hi + 1, 0};
             return Border{hk * items + hi, off - ITEM_COST};
         };
-        const long b = blockIdx.x;
-        const Border from = border(b);
-        sm.from = from;
-        sm.to = border(b + 1);
-        long first = b;
-        if (from.tile > 0) {
-            Border y;
-            do y = border(--first);
-            while (y.item == from.item && y.tile > 0);
+        // Thread 0 goes on to the CTA where the item that its border cuts begins.
+        int b = blockIdx.x + tid;
+        Border y = border(b);
+        if (tid == 1) sm.to = y;
+        else sm.from = y;
+        if (tid == 0) {
+            const Border from = y;
+#pragma unroll 1
+            while (y.tile > 0 && y.item == from.item) y = border(--b);
+            sm.first_cta = b;
+            const int e = items > 0 ? from.item % items : 0;
+            const int s = items > 0 && from.item < items * a.Hkv ? last_up_to(pl.item0, a.S, e) : 0;
+            sm.from_seq = s;
+            sm.from_i = items > 0 ? e - pl.item0[s] : 0;
+            sm.from_hk = items > 0 ? from.item / items : 0;
         }
-        sm.first_cta = static_cast<int>(first);
     }
     fence_async_smem();  // the plan's place is the copies' next
     __syncthreads();
@@ -384,15 +403,10 @@ struct LineWalker {
         k = seq_rows(p.a.cu_k, s, p.a.Nk);
         tiles = ((q.y - q.x) * p.G + ITEM_ROWS - 1) / ITEM_ROWS;
     }
-    __device__ __forceinline__ void start() {
-        if (at.item >= head_items * p.a.Hkv) return;
-        hk = at.item / head_items;
-        i = at.item % head_items;
-        load(0);
-        while (i >= tiles) {
-            i -= tiles;
-            load(s + 1);
-        }
+    __device__ __forceinline__ void start(int hk_, int seq, int i_) {
+        hk = hk_;
+        i = i_;
+        load(seq);
     }
     __device__ __forceinline__ Item next() {
         Item it;
@@ -454,31 +468,31 @@ __device__ __forceinline__ void put8(uint8_t* base, int row, int ch, const uint4
 }
 
 // Row tile t of an item's Q -> shared memory, by the 128 loader threads: rows
-// past the sequence's are zeros.
-template <class T, int D>
-__device__ __forceinline__ void load_q(const Params& p, const Item& it, int t, uint8_t* dst, int tid) {
+// past the sequence's are zeros.  The first loads are in flight while free() waits
+// for the place; false: it did not become free.
+template <class T, int D, class F>
+__device__ __forceinline__ bool load_q(const Params& p, const Item& it, int t, uint8_t* dst, int tid, F free) {
     using C = Cfg<T, D>;
     constexpr int CH = D / 8, N = BM * CH / 128, V = sizeof(T) / 2;  // chunks a row, a thread; 16-byte loads a chunk
-    constexpr int BATCH = N * V < 8 ? N : 8 / V;
+    constexpr int BATCH = N < 8 / V ? N : 8 / V;
+    static_assert(N % BATCH == 0, "whole batches");
     const uint32_t flip = p.flip ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
-    const int rows = it.nq * p.G;
+    const int r0 = it.r0 + t * BM, rows = it.nq * p.G - r0;
+    const int token0 = r0 / p.G, head0 = r0 % p.G;
+    const T* base = static_cast<const T*>(p.a.q) + static_cast<long>(it.q0 + token0) * p.a.ld_q + it.hk * p.G * D;
 #pragma unroll
     for (int b = 0; b < N; b += BATCH) {
         uint4 x[BATCH][V];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int u = tid + (b + i) * 128, r = u / CH, ch = u % CH;
-            const int row = it.r0 + t * BM + r;
-            if (row < rows) {
-                const T* src = static_cast<const T*>(p.a.q) + static_cast<long>(it.q0 + row / p.G) * p.a.ld_q +
-                               (it.hk * p.G + row % p.G) * D + ch * 8;
+            const int k = head0 + r, token = p.div(k);
+            const T* src = base + static_cast<long>(token) * p.a.ld_q + (k - token * p.G) * D + ch * 8;
 #pragma unroll
-                for (int v = 0; v < V; ++v) x[i][v] = __ldg(reinterpret_cast<const uint4*>(src) + v);
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) x[i][v] = make_uint4(0, 0, 0, 0);
-            }
+            for (int v = 0; v < V; ++v)
+                x[i][v] = r < rows ? __ldg(reinterpret_cast<const uint4*>(src) + v) : make_uint4(0, 0, 0, 0);
         }
+        if (b == 0 && !free()) return false;
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int u = tid + (b + i) * 128, r = u / CH, ch = u % CH;
@@ -488,6 +502,7 @@ __device__ __forceinline__ void load_q(const Params& p, const Item& it, int t, u
             put8<T, D, C::Q_PART, C::Q_BLOCK>(dst, r, ch, x[i][0], x[i][V - 1]);
         }
     }
+    return true;
 }
 
 // A K or V tile of f32 rows as the copy lands it (blocks of 64 columns, 32 at
@@ -532,12 +547,11 @@ __device__ __forceinline__ uint64_t k_major(uint32_t addr) {
     else return smem_desc(addr, 16, 1024);
 }
 
-// S_t = Q_t K^T of the K tile at `k`: 16 columns of d a step.
+// S = Q_t K^T of the K tile at `k`: 16 columns of d a k-step.
 template <class T, int D>
-__device__ __forceinline__ void issue_s(uint32_t tm, int t, uint32_t q, uint32_t k, uint32_t elected) {
+__device__ __forceinline__ void issue_s(uint32_t out, uint32_t q, uint32_t k, uint32_t elected) {
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, C::BN, 0, 0) : idesc_f16(BM, C::BN, 0, 0);
-    const uint32_t out = tm + C::col_s(t);
     const uint64_t qd = k_major<T, D>(q), kd = k_major<T, D>(k);
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
@@ -551,15 +565,15 @@ __device__ __forceinline__ void issue_s(uint32_t tm, int t, uint32_t q, uint32_t
     }
 }
 
-// O_t (+)= P_t V of the V tile at `v`: 16 keys a step; P's hi (and lo) words over S_t.
+// O_t (+)= P V of half h of the V tile at `v`: 16 keys a k-step; P's hi (and lo) words lie over S, at `ph`.
 template <class T, int D>
-__device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool first, uint32_t elected) {
+__device__ __forceinline__ void issue_pv(uint32_t out, uint32_t ph, uint32_t v, int h, bool first, uint32_t elected) {
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, D, 0, 1) : idesc_f16(BM, D, 0, 1);
-    const uint32_t out = tm + C::col_o(t), ph = tm + C::col_s(t);
     const uint64_t vd = D == 32 ? smem_desc_sw64(v, 512) : smem_desc(v, C::KV_BLOCK, 1024);
 #pragma unroll
-    for (int s = 0; s < C::BN / 16; ++s) {
+    for (int k = 0; k < HALF / 16; ++k) {
+        const int s = h * (HALF / 16) + k;
         const uint32_t o = s * 16 * C::ROW, ps = ph + C::col_p(s);
         mma_ts_elected(out, ps, desc_add(vd, o), id, s > 0 ? 1u : first ? 0u : 1u, elected);
         if constexpr (C::SPLIT) {
@@ -570,30 +584,31 @@ __device__ __forceinline__ void issue_pv(uint32_t tm, int t, uint32_t v, bool fi
 }
 
 // ---------------------------------------------------------------- softmax
+// The largest, or a NaN.
 template <int N>
 __device__ __forceinline__ float row_max(const float (&s)[N]) {
     float mx[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) mx[q] = fmaxf(s[q], s[q + 8]);
+    for (int q = 0; q < 8; ++q) mx[q] = max_nan(s[q], s[q + 8]);
 #pragma unroll
     for (int q = 16; q < N; q += 16)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) mx[u] = max3(mx[u], s[q + u], s[q + 8 + u]);
-    return fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7]));
+        for (int u = 0; u < 8; ++u) mx[u] = max3_nan(mx[u], s[q + u], s[q + 8 + u]);
+    return max_nan(max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3_nan(mx[5], mx[6], mx[7]));
 }
 
-// 16 columns of an output row, rounded once.
+// 32 columns of an output row, rounded once.
 template <class T>
-__device__ __forceinline__ void store16(T* out, const float (&o)[16]) {
+__device__ __forceinline__ void store32(T* out, const float (&o)[32]) {
     uint4* dst = reinterpret_cast<uint4*>(out);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 8; ++u)
             dst[u] = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]), __float_as_uint(o[4 * u + 2]),
                                 __float_as_uint(o[4 * u + 3]));
     } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 4; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
@@ -609,13 +624,9 @@ template <class T, int D>
 __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant__ Params p) {
     using C = Cfg<T, D>;
     constexpr int BN = C::BN;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Smem<T, D>& sm = *reinterpret_cast<Smem<T, D>*>(smem_raw);
+    extern __shared__ uint8_t smem_raw[];
+    Smem<T, D>& sm = *reinterpret_cast<Smem<T, D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (smem_u32(smem_raw) % 1024 != 0) {  // swizzled tiles need it; there is no room to align by hand
-        if (tid == 0) atomicOr(p.a.status, 1);
-        return;
-    }
 
     pdl_launch();
     if (warp == MMA_WARP) {
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             mbar_init(&sm.q_full[i], 128);
             mbar_init(&sm.q_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_ready[i], 8);
+            for (int h = 0; h < 2; ++h) mbar_init(&sm.p_ready[i][h], 4);
             mbar_init(&sm.o_full[i], 1);
         }
         for (int i = 0; i < C::STAGES; ++i) {
@@ -637,7 +648,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         }
         for (int i = 0; i < ITEMS; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_empty[i], 22);  // softmax 16, loader 4, MMA, TMA
+            mbar_init(&sm.item_empty[i], 14);  // softmax 8, loader 4, MMA, TMA
         }
         mbar_init(&sm.tail, 1);
         mbar_init(&sm.drain, 1);
@@ -665,73 +676,51 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
     if (warp < LOAD_WARP) {
         // ------------------------------------------------------------ softmax
         regs_to<C::R_SOFT, LAUNCH_REGS>();
-        constexpr int W = BN / 2, DW = D / 2;  // this thread's share of the keys and of O's columns
-        const int t = warp >> 3, hf = (warp >> 2) & 1;
+        const int t = warp >> 2;
         const int rl = (warp & 3) * 32 + lane;
-        const int pair = 1 + t * 4 + (warp & 3);  // named barrier of the row's two warps
         const uint32_t lb = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = lb + tm + C::col_s(t), to = lb + tm + C::col_o(t) + hf * DW;
-        int g = 0, done = 0, turn = 0;  // tiles and items of this row tile so far, exchanges
-        bool bad = false;
-        // The other thread's value; true: a wait of one of the two warps ran out (both learn it here, and leave).
-        auto exchange = [&](float mine, float& other) {
-            sm.half[turn][t][hf][rl] = mine;
-            tc_fence_before();  // this thread's reads of S come before the other's P
-            const bool stop = named_sync_or(pair, 64, bad);
-            tc_fence_after();
-            other = sm.half[turn][t][hf ^ 1][rl];
-            if constexpr (C::TURNS == 2) turn ^= 1;
-            else named_sync(pair, 64);
-            return stop;
-        };
+        const uint32_t ts = lb + tm + C::col_s(t), to = lb + tm + C::col_o(t);
+        const float slack = RESCALE_LOG2 / p.c;
+        int g = 0, done = 0;  // steps and items of this row tile so far
         for (int i = 0;; ++i) {
-            const Item& it = sm.items[i % ITEMS];  // stays in shared memory: registers are the scores'
-            bad |= !mbar_wait_warp(&sm.item_full[i % ITEMS], (i / ITEMS) & 1, limit);
-            if (named_sync_or(pair, 64, bad)) {
+            Item it;
+            if (!get_item(i, it)) {
                 failed = true;
                 break;
             }
             if (!it.valid) break;
-            auto release = [&] {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.item_empty[i % ITEMS]);
-            };
-            int seen;
-            {
-                const int row = it.r0 + t * BM + rl;
-                seen = row < it.nq * p.G ? row_seen(it.nq, it.nk, row / p.G, p.a.causal) - it.shift : 0;
-            }
+            const int row = it.r0 + t * BM + rl;
+            const bool mine = row < it.nq * p.G;
+            const int token = row / p.G;
+            const int seen = mine ? row_seen(it.nq, it.nk, token, p.a.causal) - it.shift : 0;
             const int n = it.n(t);
             float mu = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j, ++g) {
-                bad |= !mbar_wait_warp(&sm.s_full[t], g & 1, limit);
-                tc_fence_after();
-                float s[W];
-#pragma unroll
-                for (int q = 0; q < W / 32; ++q)
-                    tmem_ld32(ts + hf * W + 32 * q, reinterpret_cast<float(&)[32]>(s[32 * q]));
-                tmem_wait_ld();
-                const int lim = seen - j * BN - hf * W;  // visible columns of these
-                if (__any_sync(0xffffffffu, lim < W)) {
-#pragma unroll
-                    for (int q = 0; q < W; ++q) s[q] = q < lim ? s[q] : -INFINITY;
-                }
-                float m = row_max<W>(s), other;
-                if (exchange(m, other)) {
+                if (!mbar_wait_busy_warp(&sm.s_full[t], g & 1, limit)) {
                     failed = true;
                     break;
                 }
-                m = fmaxf(m, other);
+                tc_fence_after();
+                float s[BN];
+#pragma unroll
+                for (int q = 0; q < BN / 32; ++q) tmem_ld32(ts + 32 * q, reinterpret_cast<float(&)[32]>(s[32 * q]));
+                tmem_wait_ld();
+                const int lim = seen - j * BN;  // visible columns of these
+                if (__any_sync(0xffffffffu, lim < BN)) {
+#pragma unroll
+                    for (int q = 0; q < BN; ++q) s[q] = q < lim ? s[q] : -INFINITY;
+                }
+                const float m = row_max<BN>(s);
                 if (j == 0) {
                     mu = m;
                 } else {
-                    const bool raise = (m - mu) * p.c > RESCALE_LOG2 || (mu == -INFINITY && m > mu);
+                    const bool raise = !(m <= mu + slack);  // a NaN too
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? ex2((mu - m) * p.c) : 1.f;
                         mu = raise ? m : mu;
                         l *= f;
 #pragma unroll 1
-                        for (int q = 0; q < DW / 16; ++q) {  // few columns at a time: the scores are held meanwhile
+                        for (int q = 0; q < D / 16; ++q) {  // few columns at a time: the scores are held meanwhile
                             float o[16];
                             uint32_t r[16];
                             tmem_ld16(to + 16 * q, o);
@@ -742,97 +731,98 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         }
                     }
                 }
-                const float off = mu == -INFINITY ? 0.f : -mu * p.c;
+                // A row of nothing yet has zeros; one with an infinite score is a NaN throughout.
+                const float off = mu == -INFINITY ? 0.f : mu == INFINITY ? __uint_as_float(0x7FC00000u) : -mu * p.c;
                 const uint64_t c2 = f2_pack(p.c, p.c), off2 = f2_pack(off, off);
                 uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
-                // P over S: every column has been read (the exchange above is behind both threads' reads).
 #pragma unroll
-                for (int q = 0; q < W / 16; ++q) {
-                    uint32_t hi[8], lo[8];
+                for (int q = 0; q < BN / 32; ++q) {
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
+                    for (int u = 0; u < 16; ++u) {
+                        const uint64_t z = f2_fma(f2_pack(s[32 * q + 2 * u], s[32 * q + 2 * u + 1]), c2, off2);
                         float x, y;
-                        f2_unpack(f2_fma(f2_pack(s[16 * q + 2 * u], s[16 * q + 2 * u + 1]), c2, off2), x, y);
-                        x = ex2(x);
-                        y = ex2(y);
+                        if (!C::SPLIT && u % 8 < POLY) {
+                            exp2_poly(z, x, y);
+                        } else {
+                            f2_unpack(z, x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                        }
                         if (u & 1) sum1 = f2_add(sum1, f2_pack(x, y));
                         else sum0 = f2_add(sum0, f2_pack(x, y));
                         if constexpr (C::SPLIT) split2_x2(x, y, hi[u], lo[u]);
                         else if constexpr (C::BF16) hi[u] = pack_bf16(x, y);
                         else hi[u] = pack_f16(x, y);
                     }
-                    const uint32_t at = ts + C::col_p(hf * (W / 16) + q);
-                    tmem_st8(at, hi);
-                    if constexpr (C::SPLIT) tmem_st8(at + 16, lo);
+                    const uint32_t at = ts + C::col_p(2 * q);
+                    tmem_st16(at, hi);
+                    if constexpr (C::SPLIT) tmem_st16(at + 16, lo);
+                    if ((q + 1) % (HALF / 32) == 0) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.p_ready[t][q / (HALF / 32)]);
+                    }
                 }
                 float a0, a1;
                 f2_unpack(f2_add(sum0, sum1), a0, a1);
                 l += a0 + a1;
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_ready[t]);
             }
             if (failed) break;
-            float l2;
-            if (exchange(l, l2)) {
-                failed = true;
-                break;
-            }
-            l = hf ? l2 + l : l + l2;  // in the same order in both
             if (n > 0) {
-                bad |= !mbar_wait_warp(&sm.o_full[t], done & 1, limit);
+                if (!mbar_wait_busy_warp(&sm.o_full[t], done & 1, limit)) {
+                    failed = true;
+                    break;
+                }
                 ++done;
                 tc_fence_after();
             }
             if (it.slot >= 0) {
                 // A part: its sums as they are, columns in fours so that neighbouring rows' stores touch.
                 const int r = t * BM + rl;
-                float4* dst = p.part_o + (static_cast<long>(it.slot) * (D / 4) + hf * (DW / 4)) * ITEM_ROWS + r;
-                if (hf == 0) p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
+                float4* dst = p.part_o + static_cast<long>(it.slot) * (D / 4) * ITEM_ROWS + r;
+                p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
                 if (n > 0) {
-#pragma unroll
-                    for (int q = 0; q < DW / 16; ++q) {
-                        float o[16];
-                        tmem_ld16(to + 16 * q, o);
+#pragma unroll 1
+                    for (int q = 0; q < D / 32; ++q) {
+                        float o[32];
+                        tmem_ld32(to + 32 * q, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            dst[(4 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        for (int u = 0; u < 8; ++u)
+                            dst[(8 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                     }
                 }
-                release();
                 continue;
             }
             // Output: normalised, rounded once; rows that saw nothing are zeros.
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int row = it.r0 + t * BM + rl;
-            const bool mine = row < it.nq * p.G;
-            const int token = row / p.G, h = it.hk * p.G + row % p.G;
-            T* out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D + hf * DW;
-            if (mine && hf == 0)
+            const int h = it.hk * p.G + row % p.G;
+            T* out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D;
+            if (mine)
                 p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
                     l == 0.f ? -INFINITY : (mu * p.c + log2f(l)) * kLn2;
-#pragma unroll
-            for (int q = 0; q < DW / 16; ++q) {
-                float o[16];
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+                float o[32];
                 if (n > 0) {
-                    tmem_ld16(to + 16 * q, o);
+                    tmem_ld32(to + 32 * q, o);
                     tmem_wait_ld();
                 }
                 if (mine) {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
-                    store16<T>(out + 16 * q, o);
+                    for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
+                    store32<T>(out + 32 * q, o);
                 }
             }
-            release();
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------------------ loaders
         regs_to<C::R_LOAD, LAUNCH_REGS>();
         const int lt = tid - 32 * LOAD_WARP;
-        int used[2] = {0, 0}, kv = 0;
+        uint32_t used = 0, phase = 0;  // by row tile: whether Q_t was used before, and its phase
+        int kv = 0;
         Item it;
         for (int i = 0; !failed; ++i) {
             if (!get_item(i, it)) {
@@ -840,16 +830,20 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 break;
             }
             if (!it.valid) break;
-#pragma unroll
+#pragma unroll 1
             for (int t = 0; t < 2; ++t) {
                 if (it.n(t) == 0) continue;
                 // Q_t is free once the last S of the item that used it is done.
-                if (used[t] > 0 && !mbar_wait_warp(&sm.q_empty[t], (used[t] - 1) & 1, limit)) {
+                const bool again = (used >> t) & 1;
+                const uint32_t ph = (phase >> t) & 1;
+                if (!load_q<T, D>(p, it, t, sm.q[t], lt, [&] {
+                        return !again || mbar_wait_busy_warp(&sm.q_empty[t], ph, limit);
+                    })) {
                     failed = true;
                     break;
                 }
-                ++used[t];
-                load_q<T, D>(p, it, t, sm.q[t], lt);
+                if (again) phase ^= 1u << t;
+                used |= 1u << t;
                 fence_async_smem();
                 mbar_arrive(&sm.q_full[t]);
             }
@@ -858,10 +852,10 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 const int n = max(it.n0, it.n1);
                 for (int x = 0; x < 2 * n && !failed; ++x, ++kv) {
                     const int st = kv % C::STAGES;
-                    const bool ok = mbar_wait(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
+                    const bool ok = mbar_wait_busy(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
                     F32Tile<D> tile;
                     tile.read(sm.kv[st], it.nk - it.shift - (x >> 1) * BN, lt);
-                    if (named_sync_or(9, 128, !ok || failed)) {
+                    if (named_sync_or(1, 128, !ok || failed)) {
                         failed = true;
                         break;
                     }
@@ -879,9 +873,13 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             // uniform to the compiler too.
             const uint32_t one = elect_one();
             const uint32_t q0 = smem_u32(sm.q[0]), q1 = smem_u32(sm.q[1]), kv0 = smem_u32(sm.kv[0]);
-            int st = 0;          // ring: the next tile's stage, and its phase
-            uint32_t phase = 0;
-            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            //
+            // Per step and row tile: O += P V of the step before, then S of the step.  One copy of that code, for code
+            // size: short calls are bound by fetching instructions.
+            int st = 0;          // ring: the stage of V(j - 1), or of K(0), and its phase
+            uint32_t phase = 0, q_phase = 0, p_phase = 0;  // the latter two by row tile
+            auto stage_full = [&](int at, uint32_t ph) { return mbar_wait_busy_warp(&sm.kv_full[at], ph, limit); };
+#pragma unroll 1
             for (int i = 0; !failed; ++i) {
                 Item it;
                 if (!get_item(i, it)) {
@@ -889,51 +887,52 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     break;
                 }
                 if (!__reduce_max_sync(0xffffffffu, it.valid)) break;
-                const int nt[2] = {__reduce_max_sync(0xffffffffu, it.n0), __reduce_max_sync(0xffffffffu, it.n1)};
-                const int n = max(nt[0], nt[1]);
-                if (n == 0) continue;
-                if (!mbar_wait_warp(&sm.kv_full[st], phase, limit)) {
-                    failed = true;
-                    break;
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (failed || nt[t] == 0) continue;
-                    failed = !mbar_wait_warp(&sm.q_full[t], q_phase[t], limit);
-                    if (failed) continue;
-                    q_phase[t] ^= 1;
-                    tc_fence_after();
-                    issue_s<T, D>(tm, t, t ? q1 : q0, kv0 + st * C::KV_BYTES, one);
-                    mma_commit_elected(&sm.s_full[t], one);
-                    if (nt[t] == 1) mma_commit_elected(&sm.q_empty[t], one);
-                }
-                mma_commit_elected(&sm.kv_empty[st], one);
-                if (++st == C::STAGES) st = 0, phase ^= 1;
-                for (int j = 0; j < n && !failed; ++j) {
-                    const bool next = j + 1 < n;
-                    const int ks = st + 1 == C::STAGES ? 0 : st + 1;  // the next K tile's stage
-                    const uint32_t k_phase = ks == 0 ? phase ^ 1 : phase;
-                    failed = !mbar_wait_warp(&sm.kv_full[st], phase, limit);
-                    if (next && !failed) failed = !mbar_wait_warp(&sm.kv_full[ks], k_phase, limit);
+                const int n0 = __reduce_max_sync(0xffffffffu, it.n0), n1 = __reduce_max_sync(0xffffffffu, it.n1);
+                const int n = max(n0, n1);
+#pragma unroll 1
+                for (int j = 0; j <= n && n > 0 && !failed; ++j) {
+                    // j = 0: K(0) at st.  j > 0: V(j - 1) at st and, for j < n, K(j) behind it.
+                    int ks = st;
+                    uint32_t k_phase = phase;
+                    if (j > 0) {
+                        failed = !stage_full(st, phase);
+                        if (++ks == C::STAGES) ks = 0, k_phase ^= 1;
+                    }
+                    if (j < n && !failed) failed = !stage_full(ks, k_phase);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (failed || j >= nt[t]) continue;
-                        failed = !mbar_wait_warp(&sm.p_ready[t], p_phase[t], limit);
-                        if (failed) continue;
-                        p_phase[t] ^= 1;
-                        tc_fence_after();
-                        issue_pv<T, D>(tm, t, kv0 + st * C::KV_BYTES, j == 0, one);
-                        if (j + 1 < nt[t]) {
-                            issue_s<T, D>(tm, t, t ? q1 : q0, kv0 + ks * C::KV_BYTES, one);
+                        const int nt = t ? n1 : n0;
+                        if (failed || j > nt || nt == 0) continue;
+                        if (j > 0) {
+#pragma unroll
+                            for (int h = 0; h < C::HALVES; ++h) {
+                                if (!failed) failed = !mbar_wait_busy_warp(&sm.p_ready[t][h], (p_phase >> t) & 1, limit);
+                                if (failed) continue;
+                                tc_fence_after();
+                                issue_pv<T, D>(tm + C::col_o(t), tm + C::col_s(t), kv0 + st * C::KV_BYTES, h,
+                                               h == 0 && j == 1, one);
+                            }
+                            if (failed) continue;
+                            p_phase ^= 1u << t;
+                        } else {
+                            failed = !mbar_wait_busy_warp(&sm.q_full[t], (q_phase >> t) & 1, limit);
+                            if (failed) continue;
+                            q_phase ^= 1u << t;
+                            tc_fence_after();
+                        }
+                        if (j < nt) {
+                            issue_s<T, D>(tm + C::col_s(t), t ? q1 : q0, kv0 + ks * C::KV_BYTES, one);
                             mma_commit_elected(&sm.s_full[t], one);
-                            if (j + 2 == nt[t]) mma_commit_elected(&sm.q_empty[t], one);
+                            if (j + 1 == nt) mma_commit_elected(&sm.q_empty[t], one);
                         } else {
                             mma_commit_elected(&sm.o_full[t], one);
                         }
                     }
-                    mma_commit_elected(&sm.kv_empty[st], one);
-                    if (++st == C::STAGES) st = 0, phase ^= 1;
-                    if (next) {
+                    if (j > 0) {
+                        mma_commit_elected(&sm.kv_empty[st], one);
+                        if (++st == C::STAGES) st = 0, phase ^= 1;
+                    }
+                    if (j < n) {
                         mma_commit_elected(&sm.kv_empty[st], one);
                         if (++st == C::STAGES) st = 0, phase ^= 1;
                     }
@@ -960,7 +959,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 const int n = max(it.n0, it.n1);
                 for (int x = 0; x < 2 * n; ++x, ++kv) {
                     const int j = x >> 1, st = kv % C::STAGES, turn = kv / C::STAGES;
-                    if (turn > 0 && !mbar_wait_warp(&sm.kv_empty[st], (turn - 1) & 1, limit)) {
+                    if (turn > 0 && !mbar_wait_busy_warp(&sm.kv_empty[st], (turn - 1) & 1, limit)) {
                         failed = true;
                         break;
                     }
@@ -1003,7 +1002,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             if (p.line && lane == 0) p.joins[b].first_cta = -1;
             ItemFinder<BN> find{p.a, p.G, lane, 0, 0};
             LineWalker<BN> walk{p, sm.from, sm.to, b, sm.first_cta, sm.head_items};
-            if (p.line) walk.start();
+            if (p.line) walk.start(sm.from_hk, sm.from_seq, sm.from_i);
             else find.start();
             for (int i = 0;; ++i) {
                 const Item it = p.line ? walk.next() : find.find(i * ctas + (i & 1 ? ctas - 1 - b : b));
@@ -1082,6 +1081,7 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
     Params p{};
     p.a = a;
     p.G = a.H / a.Hkv;
+    p.inv_g = p.G > 1 ? static_cast<uint32_t>((1ull << 32) / p.G) + 1 : 0;
     // A scale of zero weighs every key alike; kept positive so that a masked score stays -inf.
     p.c = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
     p.flip = a.scale < 0.f;
@@ -1103,7 +1103,7 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
         }
     }
     auto kernel = packed_fwd<T, D>;
-    constexpr size_t smem = sizeof(Smem<T, D>);
+    constexpr size_t smem = sizeof(Smem<T, D>) + 1024;
     static_assert(smem <= SMEM_MAX, "shared memory");
     int dev = 0;
     st.cuda = cudaGetDevice(&dev);
@@ -1117,7 +1117,8 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
     }
     // Each sequence ends at most one item that is not full.
     const long head_items = static_cast<long>(a.Nq) * p.G / ITEM_ROWS + a.S;
-    p.line = head_items <= PLAN && head_items * a.Hkv < LINE_ITEMS * num_sms;
+    p.line = head_items <= PLAN && head_items * a.Hkv < LINE_ITEMS * num_sms &&
+             head_items * a.Hkv * (static_cast<long>(a.Nk) / C::BN + ITEM_COST + 1) <= INT_MAX;
     const int ctas = p.line || head_items * a.Hkv > num_sms ? num_sms : static_cast<int>(head_items * a.Hkv);
     char* ws = nullptr;
     const size_t o_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS * D, ml_bytes = sizeof(float2) * 2 * ctas * ITEM_ROWS;

@@ -145,6 +145,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
     return true;
 }
 
+// mbar_wait for hand-offs on a critical path: it polls without sleeping
+// (try_wait suspends the thread itself), in few instructions.
+__device__ __forceinline__ bool mbar_wait_busy(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity)) {
+        const uint64_t now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > limit_ns) return false;
+    }
+    return true;
+}
+__device__ __forceinline__ bool mbar_wait_busy_warp(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    return __all_sync(0xffffffffu, mbar_wait_busy(bar, parity, limit_ns));
+}
+
 // mbar_wait with a warp-uniform outcome (required before warp-collective
 // tcgen05.ld / st): true only if every lane of the warp saw the phase complete.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 1000000000ull) {
@@ -448,6 +464,42 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+// Maxima that a NaN passes through.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of both lanes on the FMA units, for where the exponential unit is the
+// bound: x = n + f with n the nearest integer (an addition of 1.5 * 2^23 rounds to it
+// and leaves it in the low bits), 2^f a polynomial of degree 5 with p(0) = 1 (minimax in
+// the relative error on [-1/2, 1/2], fitted by linear programming: 2^-22 in f32), n added to
+// the exponent.  For x <= 127; below -127 the result is 0.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
+    float x, y;
+    f2_unpack(x2, x, y);
+    x2 = f2_pack(fmaxf(x, -127.f), fmaxf(y, -127.f));
+    const uint64_t magic = f2_pack(12582912.f, 12582912.f);
+    const uint64_t n = f2_add(x2, magic);
+    const uint64_t f = f2_sub(x2, f2_sub(n, magic));
+    uint64_t p = f2_pack(0x1.5bba14p-10f, 0x1.5bba14p-10f);
+    p = f2_fma(p, f, f2_pack(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+    p = f2_fma(p, f, f2_pack(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+    p = f2_fma(p, f, f2_pack(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+    p = f2_fma(p, f, f2_pack(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+    p = f2_fma(p, f, f2_pack(1.f, 1.f));
+    float n0, n1, p0, p1;
+    f2_unpack(n, n0, n1);
+    f2_unpack(p, p0, p1);
+    a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+    b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
+
 // max(a, b, c) in one instruction (sm_100).
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
