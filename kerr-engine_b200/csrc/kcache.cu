@@ -8,187 +8,307 @@
 // odd first (truncated, its last bit set when anything was cut off), and the
 // rounding of such a number to four significant bits is that of the exact one.
 //
-// Both directions only move bytes.  A block takes a few tokens (their sequences and
-// pages are looked up once, by one thread each) and streams their heads: a
-// lane holds 16 bytes of a row, d / 4 or d / 8 lanes a row, k and v together.
+// Both directions move bytes, and are bound by the memory's rate once a row costs few
+// instructions: magnitudes are compared as integers (a NaN is larger than
+// an infinity is larger than a number; 16-bit ones two at a time), and a lane's place is kept by
+// additions.  A block streams groups of tokens, two 16-byte pieces of a row to a lane; its
+// ninth warp looks up the next group's sequences and pages (a chain of loads) meanwhile.
+#include <algorithm>
+#include <type_traits>
+
 #include "kserve.cuh"
+#include "sm100.cuh"
 
 namespace kattn {
 
 namespace {
 
 using namespace serve;
+using namespace sm100;
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 32;  // tokens of a block at most
+constexpr int kThreads = 256;   // streaming threads
+constexpr int kBlock = kThreads + 32;
+constexpr int kMaxTokens = 32;  // tokens of a group at most
+constexpr int kBlocksPerSm = 7; // resident: 32 registers a thread
 
-// Looks up tokens t0 .. t0+n-1 into shared memory: whether a sequence owns the
-// row, and the cache row of its key head 0, (page * n_kv_head) * page_size +
-// place, or -1 where there is no such row or position.
-__device__ __forceinline__ void find_places(const CacheArgs& a, int page_shift, int t0, int n, long* place, bool* owned) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+// Where a group's tokens are: the cache row of key head 0, (page * n_kv_head)
+// * page_size + place; kNowhere: no such position; kNoRow: no sequence owns the row.
+constexpr long kNowhere = -1, kNoRow = -2;
+
+__device__ __forceinline__ void find_places(const CacheArgs& a, int page_shift, int t0, int n, long* place) {
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
         const int r = t0 + i;
-        long at = -1;
-        bool mine = false;
-        if (r < a.N) {
-            const int s = seq_of_row(a.cu, a.S, r);
-            if (s >= 0) {
-                const int2 rows = seq_rows(a.cu, s, a.N);
-                if (r < rows.y) {
-                    mine = true;
-                    const int p = max(__ldg(a.kv_len + s), 0) - (rows.y - r);
-                    const int page = page_of(a, page_shift, s, p);
-                    if (page >= 0)
-                        at = (static_cast<long>(page) * a.c.n_kv_head << page_shift) + (p & (a.c.page_size - 1));
-                }
+        long at = kNoRow;
+        const int s = seq_of_row(a.cu, a.S, r);
+        if (s >= 0) {
+            const int2 rows = seq_rows(a.cu, s, a.N);
+            if (r < rows.y) {
+                const int p = max(__ldg(a.kv_len + s), 0) - (rows.y - r);
+                const int page = page_of(a, page_shift, s, p);
+                at = page < 0 ? kNowhere
+                              : (static_cast<long>(page) * a.c.n_kv_head << page_shift) + (p & (a.c.page_size - 1));
             }
         }
         place[i] = at;
-        owned[i] = mine;
     }
-    __syncthreads();
 }
 
-template <int FORMAT>
-__device__ __forceinline__ uint32_t encode(float x, float inverse) {
-    if constexpr (FORMAT == KATTN_CACHE_INT8) {
-        // |x * inverse| <= 127 (1 + 2^-23): the sum's low byte is the code.
-        return __float_as_uint(__fmaf_rn(x, inverse, 12582912.f)) & 0xFFu;
-    } else {
-        const float p = __fmul_rz(x, inverse);
-        const float rest = __fmaf_rn(x, inverse, -p);
-        const float odd = __uint_as_float(__float_as_uint(p) | (rest != 0.f ? 1u : 0u));
-        uint16_t two;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(0.f), "f"(odd));
-        return two & 0xFFu;
+// Runs stream(first token, tokens, places) over the block's groups.
+template <class F>
+__device__ __forceinline__ void for_groups(const CacheArgs& a, int page_shift, int tokens, F stream) {
+    __shared__ long place[2][kMaxTokens];
+    const int groups = (a.N + tokens - 1) / tokens;
+    int buf = 0;
+    for (int g = static_cast<int>(blockIdx.x) - static_cast<int>(gridDim.x); g < groups; g += gridDim.x, buf ^= 1) {
+        const int next = g + gridDim.x;
+        if (threadIdx.x >= kThreads) {
+            if (next < groups) find_places(a, page_shift, next * tokens, min(tokens, a.N - next * tokens), place[buf ^ 1]);
+        } else if (g >= 0) {
+            stream(g * tokens, min(tokens, a.N - g * tokens), place[buf]);
+        }
+        __syncthreads();
     }
 }
+
+// The largest magnitude among 16 bytes of T, as the bits of an f32.
+template <class T>
+__device__ __forceinline__ uint32_t magnitude(const uint4& x) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu), max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu));
+    } else {
+        const uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu),
+                                    __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+        const uint32_t h = max(m & 0xFFFFu, m >> 16);
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) return h << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+    }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void widen(const uint4& x, float (&f)[N]) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            } else {
+                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                f[2 * i] = y.x;
+                f[2 * i + 1] = y.y;
+            }
+        }
+    }
+}
+
+// Four values' codes in one word.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t encode4(const float* f, float inverse) {
+    if constexpr (FORMAT == KATTN_CACHE_INT8) {
+        // |x * inverse| <= 127 (1 + 2^-23): each sum's low byte is the code.
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(__fmaf_rn(f[i], inverse, 12582912.f));
+        return __byte_perm(__byte_perm(w[0], w[1], 0x0040u), __byte_perm(w[2], w[3], 0x0040u), 0x5410u);
+    } else {
+        float odd[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = __fmul_rz(f[i], inverse);
+            const float rest = __fmaf_rn(f[i], inverse, -p);
+            odd[i] = __uint_as_float(__float_as_uint(p) | (rest != 0.f ? 1u : 0u));
+        }
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(odd[1]), "f"(odd[0]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(odd[3]), "f"(odd[2]));
+        return lo | (static_cast<uint32_t>(hi) << 16);
+    }
+}
+
+// Four codes' values, their scale applied.
+template <int FORMAT>
+__device__ __forceinline__ void decode4(uint32_t w, float scale, float* f) {
+    if constexpr (FORMAT == KATTN_CACHE_INT8) {
+        w ^= 0x80808080u;  // code + 128, the low byte of 2^23 + 128 + code
+        const uint64_t back = f2_pack(8388736.f, 8388736.f), s2 = f2_pack(scale, scale);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float x = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u + 2 * i));
+            const float y = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441u + 2 * i));
+            f2_unpack(f2_mul(f2_sub(f2_pack(x, y), back), s2), f[2 * i], f[2 * i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t h;
+            const uint16_t two = static_cast<uint16_t>(w >> (16 * i));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            f[2 * i] = __fmul_rn(y.x, scale);
+            f[2 * i + 1] = __fmul_rn(y.y, scale);
+        }
+    }
+}
+
+// A thread's rows of the block's: row r is head r % heads of tensor (r / heads)
+// % 2 (k, v) of token r / heads / 2; the thread's are `step` apart.
+struct Walk {
+    int head, tk, heads, step_head, step_tk;
+    __device__ __forceinline__ Walk(int first, int step, int heads_)
+        : head(first % heads_), tk(first / heads_), heads(heads_), step_head(step % heads_), step_tk(step / heads_) {}
+    __device__ __forceinline__ void next() {
+        head += step_head;
+        tk += step_tk;
+        if (head >= heads) {
+            head -= heads;
+            ++tk;
+        }
+    }
+};
 
 template <class T, int FORMAT>
-__global__ void __launch_bounds__(kThreads) cache_append_rows(CacheArgs a, const T* __restrict__ k,
-                                                              const T* __restrict__ v, long ld, int page_shift,
-                                                              int tokens) {
-    constexpr int E = Vec16<T>::N;  // elements of a lane
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm) cache_append_rows(CacheArgs a, const T* __restrict__ k,
+                                                            const T* __restrict__ v, long ld, int page_shift,
+                                                            int tokens) {
+    constexpr int E = Vec16<T>::N;  // elements of a piece
     constexpr float L = FORMAT == KATTN_CACHE_INT8 ? 127.f : 448.f;
-    __shared__ long place[kMaxTokens];
-    __shared__ bool owned[kMaxTokens];
     pdl_enter();
-    const int t0 = blockIdx.x * tokens;
-    const int n = min(tokens, a.N - t0);
-    find_places(a, page_shift, t0, n, place, owned);
-    const int d = a.c.d, lanes = d / E, heads = a.c.n_kv_head;
-    const int units = n * heads * 2 * lanes;  // a multiple of `lanes`, itself a power of two up to 32
-    for (int u0 = 0; u0 < units; u0 += kThreads) {
-        const int u = u0 + threadIdx.x;
-        const bool in = u < units;
-        const int c = u % lanes, rest = u / lanes;
-        const int head = rest % heads, tk = rest / heads;
-        const int token = in ? tk >> 1 : 0;
-        const bool is_v = tk & 1;
-        const long at = in ? place[token] : -1;
-        Vec16<T> x;
-        x.raw = make_uint4(0, 0, 0, 0);
-        if (at >= 0)
-            x.raw = __ldg(reinterpret_cast<const uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld +
-                                                         head * d + c * E));
-        float f[E], m = 0.f;
-        bool nan = false;
+    const int d = a.c.d, lanes = d / (2 * E), heads = a.c.n_kv_head;  // lanes: a power of two up to 16
+    const int c = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = kThreads / lanes;
+    for_groups(a, page_shift, tokens, [&](int t0, int n, const long* place) {
+        Walk w(first, step, heads);
+        // Every thread runs as many rounds: the shuffles want whole warps.
+        for (int r = 0; r < n * heads * 2; r += step, w.next()) {
+            const int token = w.tk >> 1;
+            const bool is_v = w.tk & 1;
+            const long at = token < n ? place[token] : -1;
+            uint4 x[2];
+            x[0] = x[1] = make_uint4(0, 0, 0, 0);
+            if (at >= 0) {
+                const uint4* src = reinterpret_cast<const uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld +
+                                                                  w.head * d) + c;
+                x[0] = __ldcs(src);
+                x[1] = __ldcs(src + lanes);
+            }
+            uint32_t m = max(magnitude<T>(x[0]), magnitude<T>(x[1]));
+            for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (at < 0) continue;
+            const float most = __uint_as_float(m);
+            const bool bad = m >= 0x7F800000u, usual = !bad && most >= 0x1p-100f;
+            const float inverse = usual ? __fdiv_rn(L, most) : 0.f;
+            const long row = at + (static_cast<long>(w.head) << page_shift);
+            uint8_t* to = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            f[i] = to_f32(x.x[i]);
-            m = fmaxf(m, fabsf(f[i]));
-            nan |= f[i] != f[i];
-        }
-        if (nan) m = __uint_as_float(0x7F800000u);  // NaN and infinity alike
-        for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const bool bad = m == __uint_as_float(0x7F800000u);
-        const bool usual = !bad && m >= 0x1p-100f;
-        const float inverse = usual ? __fdiv_rn(L, m) : 0.f;
-        uint32_t w[E / 4];
+            for (int h = 0; h < 2; ++h) {
+                float f[E];
+                widen<T>(x[h], f);
+                uint32_t code[E / 4];
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) {
-            w[i] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (usual) w[i] |= encode<FORMAT>(f[4 * i + j], inverse) << (8 * j);
-        }
-        if (at >= 0) {
-            const long row = at + (static_cast<long>(head) << page_shift);
-            uint8_t* code = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
-            if constexpr (E == 4) *reinterpret_cast<uint32_t*>(code) = w[0];
-            else *reinterpret_cast<uint2*>(code) = make_uint2(w[0], w[1]);
+                for (int i = 0; i < E / 4; ++i) code[i] = usual ? encode4<FORMAT>(f + 4 * i, inverse) : 0u;
+                if constexpr (E == 4) *reinterpret_cast<uint32_t*>(to + h * lanes * E) = code[0];
+                else *reinterpret_cast<uint2*>(to + h * lanes * E) = make_uint2(code[0], code[1]);
+            }
             if (c == 0)
                 (is_v ? a.c.v_scale : a.c.k_scale)[row] =
-                    bad ? __uint_as_float(0x7FC00000u) : (usual ? __fdiv_rn(m, L) : 0.f);
+                    bad ? __uint_as_float(0x7FC00000u) : (usual ? __fdiv_rn(most, L) : 0.f);
         }
-    }
+    });
 }
 
 template <class T, int FORMAT>
-__global__ void __launch_bounds__(kThreads) cache_read_rows(CacheArgs a, T* __restrict__ k, T* __restrict__ v, long ld,
-                                                            int page_shift, int tokens) {
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm) cache_read_rows(CacheArgs a, T* __restrict__ k, T* __restrict__ v, long ld,
+                                                          int page_shift, int tokens) {
     constexpr int E = Vec16<T>::N;
-    __shared__ long place[kMaxTokens];
-    __shared__ bool owned[kMaxTokens];
+    constexpr int U = 1;  // rows of a lane at a time
     pdl_enter();
-    const int t0 = blockIdx.x * tokens;
-    const int n = min(tokens, a.N - t0);
-    find_places(a, page_shift, t0, n, place, owned);
-    const int d = a.c.d, lanes = d / E, heads = a.c.n_kv_head;
-    const int units = n * heads * 2 * lanes;
-    for (int u = threadIdx.x; u < units; u += kThreads) {
-        const int c = u % lanes, rest = u / lanes;
-        const int head = rest % heads, tk = rest / heads;
-        const int token = tk >> 1;
-        const bool is_v = tk & 1;
-        if (!owned[token]) continue;
-        const long at = place[token];
-        uint32_t w[E / 4];
+    const int d = a.c.d, lanes = d / (2 * E), heads = a.c.n_kv_head;
+    const int c = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = kThreads / lanes;
+    for_groups(a, page_shift, tokens, [&](int t0, int n, const long* place) {
+        Walk w(first, step, heads);
+        for (int r = first; r < n * heads * 2; r += U * step) {
+            uint32_t code[U][2][E / 4];
+            float scale[U];
+            uint4* to[U];
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) w[i] = 0;
-        float scale = 0.f;
-        if (at >= 0) {
-            const long row = at + (static_cast<long>(head) << page_shift);
-            const uint8_t* code = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
-            if constexpr (E == 4) {
-                w[0] = __ldg(reinterpret_cast<const uint32_t*>(code));
-            } else {
-                const uint2 t = __ldg(reinterpret_cast<const uint2*>(code));
-                w[0] = t.x;
-                w[1] = t.y;
+            for (int u = 0; u < U; ++u, w.next()) {
+                const int token = w.tk >> 1;
+                const bool is_v = w.tk & 1;
+                const long at = token < n ? place[token] : kNoRow;
+                to[u] = at != kNoRow ? reinterpret_cast<uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld +
+                                                                w.head * d) + c
+                                     : nullptr;
+                scale[u] = 0.f;
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i) code[u][0][i] = code[u][1][i] = 0;
+                if (at >= 0) {
+                    const long row = at + (static_cast<long>(w.head) << page_shift);
+                    const uint8_t* from = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (E == 4) {
+                            code[u][h][0] = __ldcs(reinterpret_cast<const uint32_t*>(from + h * lanes * E));
+                        } else {
+                            const uint2 y = __ldcs(reinterpret_cast<const uint2*>(from + h * lanes * E));
+                            code[u][h][0] = y.x;
+                            code[u][h][1] = y.y;
+                        }
+                    }
+                    scale[u] = __ldg((is_v ? a.c.v_scale : a.c.k_scale) + row);
+                }
             }
-            scale = __ldg((is_v ? a.c.v_scale : a.c.k_scale) + row);
-        }
-        Vec16<T> y;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            y.x[i] = from_f32<T>(__fmul_rn(code_value<FORMAT>((w[i / 4] >> (8 * (i % 4))) & 0xFFu), scale));
-        *reinterpret_cast<uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld + head * d + c * E) = y.raw;
-    }
+            for (int u = 0; u < U; ++u) {
+                if (!to[u]) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float f[E];
+#pragma unroll
+                    for (int i = 0; i < E / 4; ++i) decode4<FORMAT>(code[u][h][i], scale[u], f + 4 * i);
+                    uint4 y;
+                    if constexpr (sizeof(T) == 4) {
+                        y = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                       __float_as_uint(f[3]));
+                    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                        y = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
+                                       pack_bf16(f[6], f[7]));
+                    } else {
+                        y = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]),
+                                       pack_f16(f[6], f[7]));
+                    }
+                    __stcs(&to[u][h * lanes], y);
+                }
+            }
+        }
+    });
 }
 
-// Tokens of a block: as many as leave four blocks to an SM, up to kMaxTokens.
-int block_tokens(int N, int num_sms) {
+// Tokens of a group: up to 16, fewer where they would leave SMs without one; the
+// grid is as many blocks as fit at once.
+int group_tokens(int N, int num_sms) {
     int t = 1;
-    while (t < kMaxTokens && N / (2 * t) >= 4 * num_sms) t *= 2;
+    while (t < 16 && N / (2 * t) >= 2 * num_sms) t *= 2;
     return t;
 }
 
 template <class T, int FORMAT>
 ProjStatus launch_append(const CacheArgs& a, const void* k, const void* v, long ld, int num_sms, cudaStream_t s) {
-    const int tokens = block_tokens(a.N, num_sms);
+    const int tokens = group_tokens(a.N, num_sms), groups = (a.N + tokens - 1) / tokens;
     ProjStatus st;
-    st.cuda = launch_pdl(cache_append_rows<T, FORMAT>, dim3((a.N + tokens - 1) / tokens), dim3(kThreads), 0, s, a,
-                         static_cast<const T*>(k), static_cast<const T*>(v), ld, page_shift_of(a.c.page_size), tokens);
+    st.cuda = launch_pdl(cache_append_rows<T, FORMAT>, dim3(std::min(groups, kBlocksPerSm * num_sms)), dim3(kBlock), 0, s,
+                         a, static_cast<const T*>(k), static_cast<const T*>(v), ld, page_shift_of(a.c.page_size), tokens);
     st.what = "cache append launch";
     return st;
 }
 
 template <class T, int FORMAT>
 ProjStatus launch_read(const CacheArgs& a, void* k, void* v, long ld, int num_sms, cudaStream_t s) {
-    const int tokens = block_tokens(a.N, num_sms);
+    const int tokens = group_tokens(a.N, num_sms), groups = (a.N + tokens - 1) / tokens;
     ProjStatus st;
-    st.cuda = launch_pdl(cache_read_rows<T, FORMAT>, dim3((a.N + tokens - 1) / tokens), dim3(kThreads), 0, s, a,
+    st.cuda = launch_pdl(cache_read_rows<T, FORMAT>, dim3(std::min(groups, kBlocksPerSm * num_sms)), dim3(kBlock), 0, s, a,
                          static_cast<T*>(k), static_cast<T*>(v), ld, page_shift_of(a.c.page_size), tokens);
     st.what = "cache read launch";
     return st;

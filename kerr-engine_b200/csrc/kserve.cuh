@@ -14,15 +14,6 @@ namespace kattn {
 namespace serve {
 
 template <class T>
-__device__ __forceinline__ float to_f32(T x);
-template <>
-__device__ __forceinline__ float to_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
-
-template <class T>
 __device__ __forceinline__ T from_f32(float x);
 template <>
 __device__ __forceinline__ float from_f32<float>(float x) { return x; }
@@ -73,19 +64,6 @@ __host__ __device__ inline int page_shift_of(int page_size) {
     int s = 0;
     while ((1 << s) < page_size) ++s;
     return s;
-}
-
-// One 8-bit code's value.
-template <int FORMAT>
-__device__ __forceinline__ float code_value(uint32_t byte) {
-    if constexpr (FORMAT == KATTN_CACHE_INT8) {
-        return static_cast<float>(static_cast<int8_t>(byte));
-    } else {
-        // Sign, four exponent and three mantissa bits under f16's sign, five
-        // and ten: the same number times 2^-8 (subnormals included).
-        const uint16_t h = static_cast<uint16_t>(((byte & 0x80u) << 8) | ((byte & 0x7Fu) << 7));
-        return __half2float(__ushort_as_half(h)) * 256.f;
-    }
 }
 
 }  // namespace serve
