@@ -49,11 +49,11 @@ using namespace sm100;
 
 constexpr int TK = 128;              // positions of a tile
 constexpr int WARPS = 4;             // computing warps, 32 positions of a tile each
-// A warpgroup computes; of the other, a warp walks the line of work and issues the copies, one brings q into shared
-// memory, one writes results (so an item's start and end cost the computing warps little), and registers are lent.
+// A warpgroup computes; of the other, a warp walks the line of work and issues the copies, one writes results and two
+// bring q into shared memory (so an item's start and end cost the computing warps little), and registers are lent.
 // Two such CTAs to an SM.
-constexpr int N_THREADS = 256, R_COMPUTE = 208, R_SERVE = 48;
-constexpr int COPY_WARP = WARPS, Q_WARP = WARPS + 1, OUT_WARP = WARPS + 2;
+constexpr int N_THREADS = 256;
+constexpr int COPY_WARP = WARPS, OUT_WARP = WARPS + 1, Q_WARP = WARPS + 2, Q_WARPS = 2;
 constexpr int PIECES = 4;            // ring of pieces
 constexpr float RAISE = 8.f;         // a row's reference is raised when its maximum passes it by 2^8
 constexpr int EXTRA = 1;             // what an item's rows, joins and stores cost, in tiles
@@ -79,7 +79,9 @@ template <int D, int NB, bool SPLIT>
 struct Cfg {
     static constexpr int MR = 8 * NB;
     static constexpr int KS = D / 16;                          // k steps of the first product
-    static constexpr int GR = NB > 2 ? 1 : 2;                  // groups of 16 positions a warp takes at once
+    static constexpr int GR = NB * D > 256 ? 1 : 2;            // groups of 16 positions a warp takes at once (registers)
+    // Registers of a computing and of another thread: 256 together (of 128 each at launch).
+    static constexpr int R_COMPUTE = NB * D > 256 ? 216 : 184, R_SERVE = 256 - R_COMPUTE;
     static constexpr bool Q_SMEM = NB * D * (SPLIT ? 2 : 1) > 256;  // q in shared memory rather than registers
     static constexpr int Q_WORDS = KS * NB * (SPLIT ? 2 : 1) * 32;  // of a piece
     static constexpr int Q_SLOTS = Q_WORDS >= 1024 ? 1 : 2;
@@ -203,22 +205,42 @@ struct Line {
     __device__ __forceinline__ long sequence() const {
         return static_cast<long>(row_tiles) * a.cache.c.n_kv_head * (tiles + EXTRA);
     }
-    // Finds the CTA's part; whole warps.
+    // Finds the CTA's part; whole warps.  The first 128 sequences are loaded once, all at the same time.
     __device__ __forceinline__ bool start(int cta, int grid) {
-        long sum = 0;
-        for (int i = lane; i < a.cache.S; i += 32) sum += load(i);
+        constexpr int ONCE = 4;
+        const int S = a.cache.S;
+        long mine[ONCE], sum = 0;
+#pragma unroll
+        for (int c = 0; c < ONCE; ++c) mine[c] = 32 * c + lane < S ? load(32 * c + lane) : 0;
+#pragma unroll
+        for (int c = 0; c < ONCE; ++c) sum += mine[c];
+#pragma unroll 1
+        for (int i = 32 * ONCE + lane; i < S; i += 32) sum += load(i);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum;
         ctas = static_cast<int>(min(static_cast<long>(grid), total));
         if (cta >= ctas) return false;
-        at = cta * total / ctas;
-        end = (cta + 1) * total / ctas;
+        if (total <= 0x7FFFFFFFL / 1024) {  // 32-bit divisions
+            const unsigned n = static_cast<unsigned>(total), c = static_cast<unsigned>(ctas);
+            at = cta * n / c;
+            end = (cta + 1) * n / c;
+        } else {
+            at = cta * total / ctas;
+            end = (cta + 1) * total / ctas;
+        }
         long before = 0;
+#pragma unroll 1
         for (int i0 = 0;; i0 += 32) {
             const int i = i0 + lane;
-            const long mine = i < a.cache.S ? load(i) : 0;
-            long run = mine;
+            long run = 0;
+            if (i0 < 32 * ONCE) {
+#pragma unroll
+                for (int c = 0; c < ONCE; ++c) run = i0 == 32 * c ? mine[c] : run;
+            } else if (i < S) {
+                run = load(i);
+            }
+            const long own = run;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long x = __shfl_up_sync(0xffffffffu, run, o);
@@ -228,7 +250,7 @@ struct Line {
             if (hit) {
                 const int src = __ffs(hit) - 1;
                 s = i0 + src;
-                base = before + __shfl_sync(0xffffffffu, run - mine, src);
+                base = before + __shfl_sync(0xffffffffu, run - own, src);
                 break;
             }
             before += __shfl_sync(0xffffffffu, run, 31);
@@ -244,7 +266,9 @@ struct Line {
                 base += mine;
                 mine = load(++s);
             }
-            const int item = static_cast<int>((at - base) / (tiles + EXTRA));
+            const long into = at - base;
+            const int item = into <= 0x7FFFFFFFL ? static_cast<int>(into) / (tiles + EXTRA)
+                                                 : static_cast<int>(into / (tiles + EXTRA));
             p.s = s;
             p.q0 = q0;
             p.n = n;
@@ -265,7 +289,13 @@ struct Line {
         return false;
     }
     // The CTA that holds the line's tile g.
-    __device__ __forceinline__ int owner(long g) const { return static_cast<int>(((g + 1) * ctas + total - 1) / total) - 1; }
+    __device__ __forceinline__ int owner(long g) const {
+        if (total <= 0x7FFFFFFFL / 1024) {
+            const unsigned n = static_cast<unsigned>(total);
+            return static_cast<int>((static_cast<unsigned>(g + 1) * ctas + n - 1) / n) - 1;
+        }
+        return static_cast<int>(((g + 1) * ctas + total - 1) / total) - 1;
+    }
 };
 
 // ---------------------------------------------------------------- rows
@@ -322,10 +352,10 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
         }
         for (int i = 0; i < PIECES; ++i) {
             mbar_init(&sm.piece_full[i], 1);
-            mbar_init(&sm.piece_empty[i], WARPS + 2);
+            mbar_init(&sm.piece_empty[i], WARPS + 1 + Q_WARPS);
         }
         for (int i = 0; i < C::Q_SLOTS; ++i) {
-            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_full[i], Q_WARPS);
             mbar_init(&sm.q_empty[i], WARPS);
         }
         mbar_init(&sm.meet, WARPS);
@@ -354,7 +384,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     };
 
     if (warp >= WARPS) {
-        regs_dec<R_SERVE>();
+        regs_dec<C::R_SERVE>();
         if (warp == COPY_WARP) {
             // -------------------------------------------------------- the line of work, copies
             if (tid == 32 * COPY_WARP) p.joins[blockIdx.x].first_cta = -1;
@@ -422,14 +452,22 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 if (turn > 0) mbar_wait(&sm.full[st], (turn - 1) & 1, 10000000ull);
                 if (++st == C::STAGES) st = 0, ++turn;
             }
-        } else if (warp == Q_WARP) {
+        } else if (warp >= Q_WARP) {
             // -------------------------------------------------------- q
             // Operand B, row 8 nb + g: k slots (2t, 2t+1) and (2t+8, 2t+9) of step k are four neighbouring columns.
             for (int i = 0; next_piece(i); ++i) {
                 const int slot = i % C::Q_SLOTS, use = i / C::Q_SLOTS;
+                // The rows' lines start on their way before they are needed one by one.
+                for (int r = 8 * (warp - Q_WARP) + g; r < piece->rows; r += 8 * Q_WARPS) {
+                    const int row = piece->row0 + r;
+                    const long at = static_cast<long>(piece->q0 + row / p.G) * a.ld_q + (piece->hk * p.G + row % p.G) * D;
+                    const int size = a.dtype == KATTN_F32 ? 4 : 2;
+                    if (t * 128 < D * size)
+                        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(a.q) + at * size + t * 128));
+                }
                 if (use > 0 && !await(&sm.q_empty[slot], (use - 1) & 1)) return;
 #pragma unroll 1
-                for (int nb = 0; nb < NB; ++nb) {
+                for (int nb = warp - Q_WARP; nb < NB; nb += Q_WARPS) {
                     const int r = 8 * nb + g, row = piece->row0 + r;
                     const bool in = r < piece->rows;
                     const long at = static_cast<long>(piece->q0 + row / p.G) * a.ld_q + (piece->hk * p.G + row % p.G) * D;
@@ -533,7 +571,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
     }
 
     // ---------------------------------------------------------------- products
-    regs_inc<R_COMPUTE>();
+    regs_inc<C::R_COMPUTE>();
     // This lane's rows are 8 nb + 2t + c; the statistics of a row are the same in its eight lanes.
     int st = 0, turn = 0;  // ring of tiles
     uint32_t met = 0;      // meetings of the computing warps, their parity

@@ -73,7 +73,10 @@ struct Cfg {
     static constexpr int Q_BLOCK = BM * ROW, Q_PART = BLOCKS * Q_BLOCK, Q_BYTES = PARTS * Q_PART;
     // A K or V tile: per block its rows (f32: as the copy lands them, then hi rows and lo rows in their place).
     static constexpr int KV_PART = BN * ROW, KV_BLOCK = PARTS * KV_PART, KV_BYTES = BLOCKS * KV_BLOCK;
-    static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - 2 * Q_BYTES) / KV_BYTES);
+    // Output rows leave through shared memory, 64 bytes of each of a warp's 32 rows at a time, so that four lanes
+    // store one row's stretch (a lane a row takes a request each); at D = 128 the copies' stages need the place.
+    static constexpr int OUT_PITCH = 80, OUT_BYTES = D < 128 ? 8 * 32 * OUT_PITCH : 0;
+    static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - OUT_BYTES - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
     static constexpr bool BF16 = !std::is_same_v<T, __half>;
     // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
@@ -140,6 +143,7 @@ struct Smem {
     int first_cta;    // of the item that `from` cuts
     int head_items;   // items of a key head
     int from_hk, from_seq, from_i;  // the item at `from`: key head, sequence, item of the sequence
+    alignas(16) uint8_t out[C::OUT_BYTES > 0 ? C::OUT_BYTES : 16];
     uint32_t tmem_slot;
 };
 
@@ -597,18 +601,18 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
     return max_nan(max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3_nan(mx[5], mx[6], mx[7]));
 }
 
-// 32 columns of an output row, rounded once.
-template <class T>
-__device__ __forceinline__ void store32(T* out, const float (&o)[32]) {
+// N neighbouring columns of an output row, rounded once.
+template <class T, int N>
+__device__ __forceinline__ void store_row(void* out, const float (&o)[N]) {
     uint4* dst = reinterpret_cast<uint4*>(out);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < N / 4; ++u)
             dst[u] = make_uint4(__float_as_uint(o[4 * u]), __float_as_uint(o[4 * u + 1]), __float_as_uint(o[4 * u + 2]),
                                 __float_as_uint(o[4 * u + 3]));
     } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < N / 8; ++u) {
             uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x)
@@ -803,17 +807,45 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             if (mine)
                 p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
                     l == 0.f ? -INFINITY : (mu * p.c + log2f(l)) * kLn2;
-#pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-                float o[32];
-                if (n > 0) {
-                    tmem_ld32(to + 32 * q, o);
-                    tmem_wait_ld();
-                }
-                if (mine) {
+            if constexpr (C::OUT_BYTES > 0) {
+                constexpr int W = 64 / static_cast<int>(sizeof(T));  // columns of a stretch
+                uint8_t* stage = sm.out + warp * 32 * C::OUT_PITCH;
+                const uint64_t mine_at = mine ? reinterpret_cast<uint64_t>(out) : 0;
+                uint64_t at[4];  // rows 8 k + lane / 4, whose stretches this lane stores a quarter of
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
-                    store32<T>(out + 32 * q, o);
+                for (int k = 0; k < 4; ++k) at[k] = __shfl_sync(0xffffffffu, mine_at, 8 * k + (lane >> 2));
+#pragma unroll 1
+                for (int q = 0; q < D / W; ++q) {
+                    float o[W];
+                    if (n > 0) {
+                        if constexpr (W == 32) tmem_ld32(to + W * q, o);
+                        else tmem_ld16(to + W * q, o);
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int u = 0; u < W; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
+                    store_row<T, W>(stage + lane * C::OUT_PITCH, o);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(stage + (8 * k + (lane >> 2)) * C::OUT_PITCH + 16 * (lane & 3));
+                        if (at[k]) reinterpret_cast<uint4*>(at[k] + 64 * q)[lane & 3] = x;
+                    }
+                    __syncwarp();
+                }
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < D / 32; ++q) {
+                    float o[32];
+                    if (n > 0) {
+                        tmem_ld32(to + 32 * q, o);
+                        tmem_wait_ld();
+                    }
+                    if (mine) {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
+                        store_row<T, 32>(out + 32 * q, o);
+                    }
                 }
             }
         }
