@@ -83,8 +83,12 @@ struct Cfg {
     static constexpr int R_SOFT = SPLIT ? 184 : 200, R_LOAD = SPLIT ? 96 : 64, R_SERV = 48;
     static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 4 * LAUNCH_REGS, "register split");
     __host__ __device__ static constexpr uint32_t col_s(int t) { return t * BN; }
-    __host__ __device__ static constexpr uint32_t col_o(int t) { return 2 * BN + t * D; }
-    static_assert(2 * BN + 2 * D <= 512, "TMEM columns");
+    // Pairs at D <= 64: V's hi and lo are one operand of 2 D columns, and O two halves that are added at the end.  An MMA
+    // costs the same at N = 64 as at 128, so P V takes two MMAs for 16 keys instead of three.
+    static constexpr bool WIDE = SPLIT && D <= 64;
+    static constexpr int OW = WIDE ? 2 * D : D;  // TMEM columns of O
+    __host__ __device__ static constexpr uint32_t col_o(int t) { return 2 * BN + t * OW; }
+    static_assert(2 * BN + 2 * OW <= 512, "TMEM columns");
     // P's words of the 16 keys of k-step s, relative to S: packed, or, for pairs, the hi words of 32 keys and then the lo.
     __host__ __device__ static constexpr uint32_t col_p(int s) { return SPLIT ? 32 * (s >> 1) + 8 * (s & 1) : 8 * s; }
 };
@@ -275,7 +279,7 @@ struct ItemFinder {
 // Small problems: all items are one line of steps, ITEM_COST more for
 // each (its rows, its output), cut into equal parts of at least MIN_PART.  A
 // border moves to an item's edge that is near.
-constexpr int ITEM_COST = 4, MIN_PART = 6;
+constexpr int ITEM_COST = 3, MIN_PART = 5;
 constexpr long LINE_ITEMS = 6;  // items to a CTA below which a problem is small
 
 template <int BN>
@@ -354,7 +358,7 @@ __device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
     if (tid < 2) {  // the CTA's first border and its last; 32 bits hold the line (checked at launch)
         const int head = items > 0 ? pl.cost[items - 1] : 0, total = head * a.Hkv;
         const int ctas = min(static_cast<int>(gridDim.x), max(total / MIN_PART, 1));
-        const int share = total / ctas, left = total % ctas, near = share / 8 + ITEM_COST;
+        const int share = total / ctas, left = total % ctas, near = max(share / 4, 1);
         auto border = [&](int b) -> Border {
             if (b >= ctas || total == 0) return Border{items * a.Hkv, 0};
             const int at = b * share + b * left / ctas;
@@ -367,7 +371,7 @@ __device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
                 else lo = mid;
             }
             const int start = hi > 0 ? pl.cost[hi - 1] : 0, cost = pl.cost[hi] - start, off = in - start;
-            if (off <= near) return Border{hk * items + hi, 0};
+            if (off <= max(near, ITEM_COST)) return Border{hk * items + hi, 0};
             if (cost - off <= near) return Border{hk * items + hi + 1, 0};
             return Border{hk * items + hi, off - ITEM_COST};
         };
@@ -573,17 +577,16 @@ __device__ __forceinline__ void issue_s(uint32_t out, uint32_t q, uint32_t k, ui
 template <class T, int D>
 __device__ __forceinline__ void issue_pv(uint32_t out, uint32_t ph, uint32_t v, int h, bool first, uint32_t elected) {
     using C = Cfg<T, D>;
-    constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, D, 0, 1) : idesc_f16(BM, D, 0, 1);
-    const uint64_t vd = D == 32 ? smem_desc_sw64(v, 512) : smem_desc(v, C::KV_BLOCK, 1024);
+    constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, C::OW, 0, 1) : idesc_f16(BM, C::OW, 0, 1);
+    constexpr uint32_t lbo = C::WIDE ? C::KV_PART : C::KV_BLOCK;
+    const uint64_t vd = D == 32 ? smem_desc_sw64(v, 512, lbo) : smem_desc(v, lbo, 1024);
 #pragma unroll
     for (int k = 0; k < HALF / 16; ++k) {
         const int s = h * (HALF / 16) + k;
         const uint32_t o = s * 16 * C::ROW, ps = ph + C::col_p(s);
         mma_ts_elected(out, ps, desc_add(vd, o), id, s > 0 ? 1u : first ? 0u : 1u, elected);
-        if constexpr (C::SPLIT) {
-            mma_ts_elected(out, ps, desc_add(vd, o + C::KV_PART), id, 1, elected);
-            mma_ts_elected(out, ps + 16, desc_add(vd, o), id, 1, elected);
-        }
+        if constexpr (C::SPLIT && !C::WIDE) mma_ts_elected(out, ps, desc_add(vd, o + C::KV_PART), id, 1, elected);
+        if constexpr (C::SPLIT) mma_ts_elected(out, ps + 16, desc_add(vd, o), id, 1, elected);
     }
 }
 
@@ -599,6 +602,23 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) mx[u] = max3_nan(mx[u], s[q + u], s[q + 8 + u]);
     return max_nan(max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3_nan(mx[5], mx[6], mx[7]));
+}
+
+// N columns of this thread's row of O; of a wide O, the sum of its halves.
+template <bool WIDE, int D, int N>
+__device__ __forceinline__ void load_o(uint32_t at, float (&o)[N]) {
+    float y[WIDE ? N : 1];
+    if constexpr (N == 32) tmem_ld32(at, o);
+    else tmem_ld16(at, o);
+    if constexpr (WIDE) {
+        if constexpr (N == 32) tmem_ld32(at + D, y);
+        else tmem_ld16(at + D, y);
+    }
+    tmem_wait_ld();
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) o[u] += y[u];
+    }
 }
 
 // N neighbouring columns of an output row, rounded once.
@@ -724,7 +744,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         mu = raise ? m : mu;
                         l *= f;
 #pragma unroll 1
-                        for (int q = 0; q < D / 16; ++q) {  // few columns at a time: the scores are held meanwhile
+                        for (int q = 0; q < C::OW / 16; ++q) {  // few columns at a time: the scores are held meanwhile
                             float o[16];
                             uint32_t r[16];
                             tmem_ld16(to + 16 * q, o);
@@ -791,8 +811,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
 #pragma unroll 1
                     for (int q = 0; q < D / 32; ++q) {
                         float o[32];
-                        tmem_ld32(to + 32 * q, o);
-                        tmem_wait_ld();
+                        load_o<C::WIDE, D>(to + 32 * q, o);
 #pragma unroll
                         for (int u = 0; u < 8; ++u)
                             dst[(8 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
@@ -817,11 +836,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
 #pragma unroll 1
                 for (int q = 0; q < D / W; ++q) {
                     float o[W];
-                    if (n > 0) {
-                        if constexpr (W == 32) tmem_ld32(to + W * q, o);
-                        else tmem_ld16(to + W * q, o);
-                        tmem_wait_ld();
-                    }
+                    if (n > 0) load_o<C::WIDE, D>(to + W * q, o);
 #pragma unroll
                     for (int u = 0; u < W; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;
                     store_row<T, W>(stage + lane * C::OUT_PITCH, o);
@@ -837,10 +852,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
 #pragma unroll 1
                 for (int q = 0; q < D / 32; ++q) {
                     float o[32];
-                    if (n > 0) {
-                        tmem_ld32(to + 32 * q, o);
-                        tmem_wait_ld();
-                    }
+                    if (n > 0) load_o<C::WIDE, D>(to + 32 * q, o);
                     if (mine) {
 #pragma unroll
                         for (int u = 0; u < 32; ++u) o[u] = l == 0.f ? 0.f : o[u] * inv;

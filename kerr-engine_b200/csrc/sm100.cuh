@@ -276,10 +276,12 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint
 // The same for a 64-byte-swizzled K-major tile (layout type 4): rows of 64
 // bytes (32 bf16) in 8-row atoms of 512 bytes; inside an atom, row r's
 // 16-byte chunk c sits at chunk c ^ ((r >> 1) & 3).  sbo = 512.
-__device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr, uint32_t sbo) {
+// lbo (bytes) is unused for K-major tiles; for MN-major ones wider than 32 elements
+// it is the stride between 32-element column blocks.
+__device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr, uint32_t sbo, uint32_t lbo = 16) {
     uint64_t d = 0;
     d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(1u) << 16;  // leading-byte offset (unused for K-major swizzled)
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
     d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
     d |= static_cast<uint64_t>(1u) << 46;  // version
     d |= static_cast<uint64_t>(4u) << 61;  // SWIZZLE_64B
