@@ -81,7 +81,7 @@ struct Cfg {
     static constexpr int KS = D / 16;                          // k steps of the first product
     static constexpr int GR = NB * D > 256 ? 1 : 2;            // groups of 16 positions a warp takes at once (registers)
     // Registers of a computing and of another thread: 256 together (of 128 each at launch).
-    static constexpr int R_COMPUTE = NB * D > 256 ? 216 : 184, R_SERVE = 256 - R_COMPUTE;
+    static constexpr int R_COMPUTE = NB * D > 256 ? 224 : 184, R_SERVE = 256 - R_COMPUTE;
     static constexpr bool Q_SMEM = NB * D * (SPLIT ? 2 : 1) > 256;  // q in shared memory rather than registers
     static constexpr int Q_WORDS = KS * NB * (SPLIT ? 2 : 1) * 32;  // of a piece
     static constexpr int Q_SLOTS = Q_WORDS >= 1024 ? 1 : 2;

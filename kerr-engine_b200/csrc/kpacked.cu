@@ -120,7 +120,7 @@ struct Border {
 
 // Small problems: the items of one key head and their running cost, while a
 // CTA looks for its part of the line.
-constexpr int PLAN = 1024;
+constexpr int PLAN = N_THREADS;
 struct Plan {
     int2 seq[PLAN];   // rows and keys of each sequence
     int item0[PLAN];  // its first item
@@ -288,23 +288,19 @@ __device__ __forceinline__ int item_cost(int2 seq, int G, int causal, int item) 
     return ITEM_COST + max(key_tiles<BN>(seq.x, seq.y, G, causal, r), key_tiles<BN>(seq.x, seq.y, G, causal, r + BM));
 }
 
-// Running sums of x0, x1 (elements 2 tid and 2 tid + 1) over the block's threads.
-__device__ __forceinline__ void block_scan(int& x0, int& x1, int* warp_sum, int tid) {
+// Running sum of x over the block's threads.
+__device__ __forceinline__ int block_scan(int x, int* warp_sum, int tid) {
     const int lane = tid & 31;
-    const int own = x0 + x1;
-    int sum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
     }
-    if (lane == 31) warp_sum[tid >> 5] = sum;
+    if (lane == 31) warp_sum[tid >> 5] = x;
     __syncthreads();
-    int before = lane < (tid >> 5) ? warp_sum[lane] : 0;
-    before = __reduce_add_sync(0xffffffffu, before);
+    const int before = __reduce_add_sync(0xffffffffu, lane < (tid >> 5) ? warp_sum[lane] : 0);
     __syncthreads();
-    x0 += before + sum - own;
-    x1 += x0;
+    return x + before;
 }
 
 // The last element of the ascending v[0 .. n-1] that is <= x (v[0] is).
@@ -324,36 +320,24 @@ template <int BN, class S>
 __device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
     const PackedArgs& a = p.a;
     Plan& pl = sm.plan;
-    int x[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int s = 2 * tid + u;
-        x[u] = 0;
-        if (s < a.S) {
-            const int2 q = seq_rows(a.cu_q, s, a.Nq), k = seq_rows(a.cu_k, s, a.Nk);
-            pl.seq[s] = make_int2(q.y - q.x, k.y - k.x);
-            x[u] = ((q.y - q.x) * p.G + ITEM_ROWS - 1) / ITEM_ROWS;
-        }
+    int own = 0;
+    if (tid < a.S) {
+        const int2 q = seq_rows(a.cu_q, tid, a.Nq), k = seq_rows(a.cu_k, tid, a.Nk);
+        pl.seq[tid] = make_int2(q.y - q.x, k.y - k.x);
+        own = ((q.y - q.x) * p.G + ITEM_ROWS - 1) / ITEM_ROWS;
     }
-    const int own0 = x[0], own1 = x[1];
-    block_scan(x[0], x[1], pl.warp_sum, tid);
-    if (2 * tid < a.S) pl.item0[2 * tid] = x[0] - own0;
-    if (2 * tid + 1 < a.S) pl.item0[2 * tid + 1] = x[1] - own1;
-    if (tid == N_THREADS - 1) sm.head_items = x[1];
+    int sum = block_scan(own, pl.warp_sum, tid);
+    if (tid < a.S) pl.item0[tid] = sum - own;
+    if (tid == N_THREADS - 1) sm.head_items = sum;
     __syncthreads();
     const int items = sm.head_items;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int e = 2 * tid + u;
-        x[u] = 0;
-        if (e < items) {
-            const int s = last_up_to(pl.item0, a.S, e);
-            x[u] = item_cost<BN>(pl.seq[s], p.G, a.causal, e - pl.item0[s]);
-        }
+    own = 0;
+    if (tid < items) {
+        const int s = last_up_to(pl.item0, a.S, tid);
+        own = item_cost<BN>(pl.seq[s], p.G, a.causal, tid - pl.item0[s]);
     }
-    block_scan(x[0], x[1], pl.warp_sum, tid);
-    if (2 * tid < items) pl.cost[2 * tid] = x[0];
-    if (2 * tid + 1 < items) pl.cost[2 * tid + 1] = x[1];
+    sum = block_scan(own, pl.warp_sum, tid);
+    if (tid < items) pl.cost[tid] = sum;
     __syncthreads();
     if (tid < 2) {  // the CTA's first border and its last; 32 bits hold the line (checked at launch)
         const int head = items > 0 ? pl.cost[items - 1] : 0, total = head * a.Hkv;
