@@ -410,8 +410,10 @@ int kattn_block_bwd(kattn_ctx* ctx, kattn_block* blk, const float* dh_out, float
  * there and never synchronise the host.
  *
  * Types.  dtype names the element type of q, k, v and o: scores, softmax
- * statistics and sums are formed in f32 (in bf16 hi/lo or f16 hi/lo products,
- * about 1e-5, for KATTN_F32), and outputs are rounded once.  Device pointers
+ * statistics and sums are formed in f32, and outputs are rounded once.  Products
+ * of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about 1e-6,
+ * with 2^-37 of the largest magnitude among a sequence's rows as the least step.
+ * Sums of v are formed before they are divided: |v| is to stay below 2^96.  Device pointers
  * are 16-byte aligned and row strides a multiple of 16 bytes; int32 arrays
  * and lse 4-byte, tree 8-byte aligned.  d is 32, 64 or 128.
  *

@@ -18,7 +18,7 @@
 //
 // Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
 // one thread a row.  8-11: Q into shared memory (and, for f32, K and V split
-// in place into bf16 hi and lo).  12: issues every MMA.  13: TMA of K and V.  14: walks
+// in place into hi and lo).  12: issues every MMA.  13: TMA of K and V.  14: walks
 // the CTA's work.
 //
 // Steps of 128 keys (64 for f32 at D = 128).  While one row tile is in its softmax,
@@ -29,8 +29,11 @@
 // being the larger read.)  TMEM: 2 x 128 columns of S and P, 2 x D of O, 512 at D = 128.
 //
 // Types.  16-bit operands enter the MMAs as they are and P is rounded to the type; f32
-// ones as bf16 pairs, hi*hi + hi*lo + lo*hi (about 2^-17 of a product, where one
-// TF32 product would be off by 2^-11).
+// ones as f16 pairs (22 bits), hi*hi + hi*lo + lo*hi, after powers of two have brought
+// them near 2^14: one a row of Q, one a tile of K, one for the V tiles of an item (it
+// rises when one needs it, and O follows).  They go back in with the exponent's factor
+// and the output.  bf16 pairs need no powers and took 84 us where this takes 93 (chunks
+// over cached contexts, f32), but are off by 6e-6; these by 3e-7 to 9e-7, as an f32 product is.
 //
 // Weights are 2^(c s - c mu), c = scale log2(e), with mu raised only when a
 // tile's maximum passes it by more than 2^8 (then O and the sum are scaled): weights
@@ -58,13 +61,14 @@ constexpr int N_THREADS = 512, LAUNCH_REGS = 128;
 constexpr int LOAD_WARP = 8, MMA_WARP = 12, TMA_WARP = 13, ITEM_WARP = 14;
 constexpr int ITEMS = 4;         // item ring
 constexpr float RESCALE_LOG2 = 8.f;
+constexpr int UNITS = 16;       // ring of the K and V tiles' powers of two: more than tiles can be under way
 constexpr int POLY = 1;          // of 8 pairs of weights by the FMA units (16-bit types)
 constexpr uint32_t TMEM_COLS = 512;
 constexpr size_t SMEM_MAX = 227 * 1024;
 
 template <class T, int D>
 struct Cfg {
-    static constexpr bool SPLIT = sizeof(T) == 4;            // operands as bf16 hi / lo pairs
+    static constexpr bool SPLIT = sizeof(T) == 4;            // operands as f16 hi / lo pairs
     static constexpr int PARTS = SPLIT ? 2 : 1;
     static constexpr int BN = SPLIT && D == 128 ? 64 : 128;  // keys of a step (64: Q's pairs leave less room)
     static constexpr int HALVES = BN / HALF;
@@ -78,7 +82,8 @@ struct Cfg {
     static constexpr int OUT_PITCH = 80, OUT_BYTES = D < 128 ? 8 * 32 * OUT_PITCH : 0;
     static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - OUT_BYTES - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
-    static constexpr bool BF16 = !std::is_same_v<T, __half>;
+    static constexpr bool BF16 = std::is_same_v<T, __nv_bfloat16>;  // the operands' type; else f16
+    static constexpr float W_UP = SPLIT ? 7.f : 0.f;  // weights are held times 2^7 (then at most 2^15), far from f16's subnormals
     // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
     static constexpr int R_SOFT = SPLIT ? 184 : 200, R_LOAD = SPLIT ? 96 : 64, R_SERV = 48;
     static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 4 * LAUNCH_REGS, "register split");
@@ -147,6 +152,9 @@ struct Smem {
     int first_cta;    // of the item that `from` cuts
     int head_items;   // items of a key head
     int from_hk, from_seq, from_i;  // the item at `from`: key head, sequence, item of the sequence
+    uint8_t unit_q[2][2][BM];   // f32: the exponents that go back into Q's rows, by row tile, of its items in turn
+    float unit_kv[UNITS];      // and the factors of the K and V tiles, in their order
+    uint32_t most[2][4];         // the loader warps' largest magnitudes of a tile
     alignas(16) uint8_t out[C::OUT_BYTES > 0 ? C::OUT_BYTES : 16];
     uint32_t tmem_slot;
 };
@@ -160,7 +168,7 @@ struct Params {
     int flip;  // scale < 0: the rows of Q are negated
     int line;  // a small problem
     float4* part_o;   // [2 * CTAs][D / 4][256 rows]: a CTA's part that began before it (0) or begins in it (1)
-    float2* part_ml;  // [2 * CTAs][256 rows]: row maxima (times c) and sums
+    float* part_lse;  // [2 * CTAs][256 rows]: log2 of the rows' sums
     Join* joins;      // [CTAs]
     // x / G for x below 2^32 / G (the product is off by less than x G / 2^32).
     __device__ __forceinline__ int div(int x) const { return G == 1 ? x : static_cast<int>(__umulhi(x, inv_g)); }
@@ -442,16 +450,17 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {  // 16-byte c
 }
 
 // 8 values of a row -> the operand's bytes at (row, 8-column chunk ch): one
-// 16-byte chunk, two (hi, lo) for f32.
+// 16-byte chunk, two (hi, lo, times `up`) for f32.
 template <class T, int D, int PART, int BLOCK>
-__device__ __forceinline__ void put8(uint8_t* base, int row, int ch, const uint4& x0, const uint4& x1) {
+__device__ __forceinline__ void put8(uint8_t* base, int row, int ch, const uint4& x0, const uint4& x1, float up) {
     uint8_t* at = base + (ch >> 3) * BLOCK + swizzled<T, D>(row, ch & 7);
     if constexpr (sizeof(T) == 4) {
         uint4 hi, lo;
-        split2(__uint_as_float(x0.x), __uint_as_float(x0.y), hi.x, lo.x);
-        split2(__uint_as_float(x0.z), __uint_as_float(x0.w), hi.y, lo.y);
-        split2(__uint_as_float(x1.x), __uint_as_float(x1.y), hi.z, lo.z);
-        split2(__uint_as_float(x1.z), __uint_as_float(x1.w), hi.w, lo.w);
+        const uint64_t up2 = f2_pack(up, up);
+        split2_f16(f2_mul(f2_pack(__uint_as_float(x0.x), __uint_as_float(x0.y)), up2), hi.x, lo.x);
+        split2_f16(f2_mul(f2_pack(__uint_as_float(x0.z), __uint_as_float(x0.w)), up2), hi.y, lo.y);
+        split2_f16(f2_mul(f2_pack(__uint_as_float(x1.x), __uint_as_float(x1.y)), up2), hi.z, lo.z);
+        split2_f16(f2_mul(f2_pack(__uint_as_float(x1.z), __uint_as_float(x1.w)), up2), hi.w, lo.w);
         *reinterpret_cast<uint4*>(at) = hi;
         *reinterpret_cast<uint4*>(at + PART) = lo;
     } else {
@@ -463,7 +472,7 @@ __device__ __forceinline__ void put8(uint8_t* base, int row, int ch, const uint4
 // past the sequence's are zeros.  The first loads are in flight while free() waits
 // for the place; false: it did not become free.
 template <class T, int D, class F>
-__device__ __forceinline__ bool load_q(const Params& p, const Item& it, int t, uint8_t* dst, int tid, F free) {
+__device__ __forceinline__ bool load_q(const Params& p, const Item& it, int t, uint8_t* dst, uint8_t* unit_q, int tid, F free) {
     using C = Cfg<T, D>;
     constexpr int CH = D / 8, N = BM * CH / 128, V = sizeof(T) / 2;  // chunks a row, a thread; 16-byte loads a chunk
     constexpr int BATCH = N < 8 / V ? N : 8 / V;
@@ -491,14 +500,27 @@ __device__ __forceinline__ bool load_q(const Params& p, const Item& it, int t, u
 #pragma unroll
             for (int v = 0; v < V; ++v)
                 x[i][v] = make_uint4(x[i][v].x ^ flip, x[i][v].y ^ flip, x[i][v].z ^ flip, x[i][v].w ^ flip);
-            put8<T, D, C::Q_PART, C::Q_BLOCK>(dst, r, ch, x[i][0], x[i][V - 1]);
+            float up = 1.f;
+            if constexpr (C::SPLIT) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    most = max(most, max(max(x[i][v].x & 0x7FFFFFFFu, x[i][v].y & 0x7FFFFFFFu),
+                                         max(x[i][v].z & 0x7FFFFFFFu, x[i][v].w & 0x7FFFFFFFu)));
+#pragma unroll
+                for (int o = CH / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float unit = unit_2_14(most);
+                up = inverse_of_power(unit);
+                if (ch == 0) unit_q[r] = static_cast<uint8_t>(__float_as_uint(unit) >> 23);
+            }
+            put8<T, D, C::Q_PART, C::Q_BLOCK>(dst, r, ch, x[i][0], x[i][V - 1], up);
         }
     }
     return true;
 }
 
 // A K or V tile of f32 rows as the copy lands it (blocks of 64 columns, 32 at
-// D = 32, row-major) -> the same bytes as swizzled bf16 hi rows and lo rows, by the
+// D = 32, row-major) -> the same bytes as swizzled f16 hi rows and lo rows, by the
 // 128 loader threads: all read before any writes.  Rows from `rows` on, the next
 // sequence's, become zeros: their weights are zero, and zero times an infinity is not.
 template <int D>
@@ -517,15 +539,27 @@ struct F32Tile {
                 if (f / Q4 >= rows) x[b][i] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
     }
-    __device__ __forceinline__ void write(uint8_t* tile, int tid) const {
+    __device__ __forceinline__ uint32_t most() const {  // the bits of the largest magnitude but NaN
+        float m = 0.f;
+#pragma unroll
+        for (int b = 0; b < C::BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                m = fmaxf(m, fmaxf(fabsf(x[b][i].x), fabsf(x[b][i].y)));
+                m = fmaxf(m, fmaxf(fabsf(x[b][i].z), fabsf(x[b][i].w)));
+            }
+        return __float_as_uint(m);
+    }
+    __device__ __forceinline__ void write(uint8_t* tile, float up, int tid) const {
+        const uint64_t up2 = f2_pack(up, up);
 #pragma unroll
         for (int b = 0; b < C::BLOCKS; ++b)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int f = tid + i * 128, r = f / Q4, c4 = f % Q4;
                 uint2 h, l;
-                split2_x2(x[b][i].x, x[b][i].y, h.x, l.x);
-                split2_x2(x[b][i].z, x[b][i].w, h.y, l.y);
+                split2_f16(f2_mul(f2_pack(x[b][i].x, x[b][i].y), up2), h.x, l.x);
+                split2_f16(f2_mul(f2_pack(x[b][i].z, x[b][i].w), up2), h.y, l.y);
                 uint8_t* at = tile + b * C::KV_BLOCK + swizzled<float, D>(r, c4 >> 1) + (c4 & 1) * 8;
                 *reinterpret_cast<uint2*>(at) = h;
                 *reinterpret_cast<uint2*>(at + C::KV_PART) = l;
@@ -545,23 +579,25 @@ __device__ __forceinline__ void issue_s(uint32_t out, uint32_t q, uint32_t k, ui
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, C::BN, 0, 0) : idesc_f16(BM, C::BN, 0, 0);
     const uint64_t qd = k_major<T, D>(q), kd = k_major<T, D>(k);
+    // The products with a lo first: each sum is rounded to the size that it has by then.
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-        const uint32_t qo = (s >> 2) * C::Q_BLOCK + (s & 3) * 32, ko = (s >> 2) * C::KV_BLOCK + (s & 3) * 32;
-        if (s == 0) mma_ss_elected<false>(out, qd, kd, id, elected);
-        else mma_ss_elected<true>(out, desc_add(qd, qo), desc_add(kd, ko), id, elected);
-        if constexpr (C::SPLIT) {
-            mma_ss_elected<true>(out, desc_add(qd, qo), desc_add(kd, ko + C::KV_PART), id, elected);
-            mma_ss_elected<true>(out, desc_add(qd, qo + C::Q_PART), desc_add(kd, ko), id, elected);
+    for (int part = C::SPLIT ? 2 : 0; part >= 0; --part)
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            const uint32_t qo = (s >> 2) * C::Q_BLOCK + (s & 3) * 32 + (part == 2 ? C::Q_PART : 0);
+            const uint32_t ko = (s >> 2) * C::KV_BLOCK + (s & 3) * 32 + (part == 1 ? C::KV_PART : 0);
+            if (s == 0 && part == (C::SPLIT ? 2 : 0)) mma_ss_elected<false>(out, desc_add(qd, qo), desc_add(kd, ko), id, elected);
+            else mma_ss_elected<true>(out, desc_add(qd, qo), desc_add(kd, ko), id, elected);
         }
-    }
 }
 
-// O_t (+)= P V of half h of the V tile at `v`: 16 keys a k-step; P's hi (and lo) words lie over S, at `ph`.
+// O_t (+)= P V of half h of the V tile at `v`: 16 keys a k-step; P's hi (and lo) words lie over S, at `ph`.  Of a
+// wide O the first half takes hi hi, the second the products with a lo, so that the larger is rounded less often.
 template <class T, int D>
 __device__ __forceinline__ void issue_pv(uint32_t out, uint32_t ph, uint32_t v, int h, bool first, uint32_t elected) {
     using C = Cfg<T, D>;
     constexpr uint32_t id = C::BF16 ? idesc_bf16(BM, C::OW, 0, 1) : idesc_f16(BM, C::OW, 0, 1);
+    constexpr uint32_t id_lo = idesc_f16(BM, D, 0, 1), to_lo = C::WIDE ? D : 0;
     constexpr uint32_t lbo = C::WIDE ? C::KV_PART : C::KV_BLOCK;
     const uint64_t vd = D == 32 ? smem_desc_sw64(v, 512, lbo) : smem_desc(v, lbo, 1024);
 #pragma unroll
@@ -570,11 +606,26 @@ __device__ __forceinline__ void issue_pv(uint32_t out, uint32_t ph, uint32_t v, 
         const uint32_t o = s * 16 * C::ROW, ps = ph + C::col_p(s);
         mma_ts_elected(out, ps, desc_add(vd, o), id, s > 0 ? 1u : first ? 0u : 1u, elected);
         if constexpr (C::SPLIT && !C::WIDE) mma_ts_elected(out, ps, desc_add(vd, o + C::KV_PART), id, 1, elected);
-        if constexpr (C::SPLIT) mma_ts_elected(out, ps + 16, desc_add(vd, o), id, 1, elected);
+        if constexpr (C::SPLIT) mma_ts_elected(out + to_lo, ps + 16, desc_add(vd, o), id_lo, 1, elected);
     }
 }
 
 // ---------------------------------------------------------------- softmax
+// O's columns times f, few at a time: the scores are held meanwhile.
+template <int N>
+__device__ __forceinline__ void scale_o(uint32_t at, float f) {
+#pragma unroll 1
+    for (int q = 0; q < N; q += 16) {
+        float o[16];
+        uint32_t r[16];
+        tmem_ld16(at + q, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int u = 0; u < 16; ++u) r[u] = __float_as_uint(o[u] * f);
+        tmem_st16(at + q, r);
+    }
+}
+
 // The largest, or a NaN.
 template <int N>
 __device__ __forceinline__ float row_max(const float (&s)[N]) {
@@ -688,8 +739,8 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         const int rl = (warp & 3) * 32 + lane;
         const uint32_t lb = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = lb + tm + C::col_s(t), to = lb + tm + C::col_o(t);
-        const float slack = RESCALE_LOG2 / p.c;
         int g = 0, done = 0;  // steps and items of this row tile so far
+        int kv = 0;           // f32: K and V tiles before the item's
         for (int i = 0;; ++i) {
             Item it;
             if (!get_item(i, it)) {
@@ -702,7 +753,9 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             const int token = row / p.G;
             const int seen = mine ? row_seen(it.nq, it.nk, token, p.a.causal) - it.shift : 0;
             const int n = it.n(t);
-            float mu = -INFINITY, l = 0.f;
+            float mu = -INFINITY, l = 0.f;  // mu in the exponent's units
+            float c = p.c;     // f32: times the power of two of the row of Q
+            float unit = 1.f;  // f32: the power of two that V and O are counted in
             for (int j = 0; j < n; ++j, ++g) {
                 if (!mbar_wait_busy_warp(&sm.s_full[t], g & 1, limit)) {
                     failed = true;
@@ -718,30 +771,26 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
 #pragma unroll
                     for (int q = 0; q < BN; ++q) s[q] = q < lim ? s[q] : -INFINITY;
                 }
-                const float m = row_max<BN>(s);
+                float cs = c;
+                if constexpr (C::SPLIT) {
+                    if (j == 0) c = p.c * __uint_as_float(static_cast<uint32_t>(sm.unit_q[t][done & 1][rl]) << 23);
+                    cs = fmaxf(c * sm.unit_kv[(kv + 2 * j) % UNITS], 1e-37f);  // positive: a masked score stays -inf
+                }
+                const float m = row_max<BN>(s) * cs;
+                float f = 1.f;  // for O, before this step's products join it
                 if (j == 0) {
                     mu = m;
                 } else {
-                    const bool raise = !(m <= mu + slack);  // a NaN too
+                    const bool raise = !(m <= mu + RESCALE_LOG2);  // a NaN too
                     if (__any_sync(0xffffffffu, raise)) {
-                        const float f = raise ? ex2((mu - m) * p.c) : 1.f;
+                        f = raise ? ex2(mu - m) : 1.f;
                         mu = raise ? m : mu;
                         l *= f;
-#pragma unroll 1
-                        for (int q = 0; q < C::OW / 16; ++q) {  // few columns at a time: the scores are held meanwhile
-                            float o[16];
-                            uint32_t r[16];
-                            tmem_ld16(to + 16 * q, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int u = 0; u < 16; ++u) r[u] = __float_as_uint(o[u] * f);
-                            tmem_st16(to + 16 * q, r);
-                        }
                     }
                 }
                 // A row of nothing yet has zeros; one with an infinite score is a NaN throughout.
-                const float off = mu == -INFINITY ? 0.f : mu == INFINITY ? __uint_as_float(0x7FC00000u) : -mu * p.c;
-                const uint64_t c2 = f2_pack(p.c, p.c), off2 = f2_pack(off, off);
+                const float off = mu == -INFINITY ? 0.f : mu == INFINITY ? __uint_as_float(0x7FC00000u) : C::W_UP - mu;
+                const uint64_t c2 = f2_pack(cs, cs), off2 = f2_pack(off, off);
                 uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
 #pragma unroll
                 for (int q = 0; q < BN / 32; ++q) {
@@ -759,7 +808,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         }
                         if (u & 1) sum1 = f2_add(sum1, f2_pack(x, y));
                         else sum0 = f2_add(sum0, f2_pack(x, y));
-                        if constexpr (C::SPLIT) split2_x2(x, y, hi[u], lo[u]);
+                        if constexpr (C::SPLIT) split2_f16(f2_pack(x, y), hi[u], lo[u]);
                         else if constexpr (C::BF16) hi[u] = pack_bf16(x, y);
                         else hi[u] = pack_f16(x, y);
                     }
@@ -767,6 +816,17 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     tmem_st16(at, hi);
                     if constexpr (C::SPLIT) tmem_st16(at + 16, lo);
                     if ((q + 1) % (HALF / 32) == 0) {
+                        if constexpr (C::SPLIT) {
+                            // V's unit may have risen.
+                            if (q == HALF / 32 - 1) {
+                                const int x = kv + 2 * j + 1;
+                                if (!mbar_wait_busy_warp(&sm.kv_full[x % C::STAGES], x / C::STAGES & 1, limit)) failed = true;
+                                const float now = sm.unit_kv[x % UNITS];
+                                if (j > 0) f *= unit * inverse_of_power(now);
+                                unit = now;
+                            }
+                        }
+                        if (q == HALF / 32 - 1 && __any_sync(0xffffffffu, f != 1.f)) scale_o<C::OW>(to, f);
                         tmem_wait_st();
                         tc_fence_before();
                         __syncwarp();
@@ -776,8 +836,10 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 float a0, a1;
                 f2_unpack(f2_add(sum0, sum1), a0, a1);
                 l += a0 + a1;
+                if (failed) break;
             }
             if (failed) break;
+            kv += 2 * max(it.n0, it.n1);
             if (n > 0) {
                 if (!mbar_wait_busy_warp(&sm.o_full[t], done & 1, limit)) {
                     failed = true;
@@ -786,11 +848,13 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 ++done;
                 tc_fence_after();
             }
+            const float inv = l == 0.f ? 0.f : unit / l;
+            const float lse = l == 0.f ? -INFINITY : mu - C::W_UP + log2f(l);
             if (it.slot >= 0) {
-                // A part: its sums as they are, columns in fours so that neighbouring rows' stores touch.
+                // A part: normalised, columns in fours so that neighbouring rows' stores touch.
                 const int r = t * BM + rl;
                 float4* dst = p.part_o + static_cast<long>(it.slot) * (D / 4) * ITEM_ROWS + r;
-                p.part_ml[static_cast<long>(it.slot) * ITEM_ROWS + r] = make_float2(mu * p.c, l);
+                p.part_lse[static_cast<long>(it.slot) * ITEM_ROWS + r] = lse;
                 if (n > 0) {
 #pragma unroll 1
                     for (int q = 0; q < D / 32; ++q) {
@@ -798,18 +862,17 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         load_o<C::WIDE, D>(to + 32 * q, o);
 #pragma unroll
                         for (int u = 0; u < 8; ++u)
-                            dst[(8 * q + u) * ITEM_ROWS] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                            dst[(8 * q + u) * ITEM_ROWS] =
+                                make_float4(o[4 * u] * inv, o[4 * u + 1] * inv, o[4 * u + 2] * inv, o[4 * u + 3] * inv);
                     }
                 }
                 continue;
             }
             // Output: normalised, rounded once; rows that saw nothing are zeros.
-            const float inv = l == 0.f ? 0.f : 1.f / l;
             const int h = it.hk * p.G + row % p.G;
             T* out = static_cast<T*>(p.a.o) + static_cast<long>(it.q0 + token) * p.a.ld_o + h * D;
             if (mine)
-                p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] =
-                    l == 0.f ? -INFINITY : (mu * p.c + log2f(l)) * kLn2;
+                p.a.lse[static_cast<long>(h) * p.a.Nq + it.q0 + token] = lse * kLn2;
             if constexpr (C::OUT_BYTES > 0) {
                 constexpr int W = 64 / static_cast<int>(sizeof(T));  // columns of a stretch
                 uint8_t* stage = sm.out + warp * 32 * C::OUT_PITCH;
@@ -849,7 +912,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
         // ------------------------------------------------------------ loaders
         regs_to<C::R_LOAD, LAUNCH_REGS>();
         const int lt = tid - 32 * LOAD_WARP;
-        uint32_t used = 0, phase = 0;  // by row tile: whether Q_t was used before, and its phase
+        uint32_t used = 0, phase = 0, turn = 0;  // by row tile: whether Q_t was used before, its phase, its scales' turn
         int kv = 0;
         Item it;
         for (int i = 0; !failed; ++i) {
@@ -864,7 +927,7 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 // Q_t is free once the last S of the item that used it is done.
                 const bool again = (used >> t) & 1;
                 const uint32_t ph = (phase >> t) & 1;
-                if (!load_q<T, D>(p, it, t, sm.q[t], lt, [&] {
+                if (!load_q<T, D>(p, it, t, sm.q[t], sm.unit_q[t][turn >> t & 1], lt, [&] {
                         return !again || mbar_wait_busy_warp(&sm.q_empty[t], ph, limit);
                     })) {
                     failed = true;
@@ -872,22 +935,30 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                 }
                 if (again) phase ^= 1u << t;
                 used |= 1u << t;
+                turn ^= 1u << t;
                 fence_async_smem();
                 mbar_arrive(&sm.q_full[t]);
             }
             if constexpr (C::SPLIT) {
                 // K_0, V_0, K_1, ...: each converted in place once it has landed.
                 const int n = max(it.n0, it.n1);
+                float unit_v = 0.f;  // rises only, with room for V tiles up to four times the first
                 for (int x = 0; x < 2 * n && !failed; ++x, ++kv) {
                     const int st = kv % C::STAGES;
                     const bool ok = mbar_wait_busy(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
                     F32Tile<D> tile;
                     tile.read(sm.kv[st], it.nk - it.shift - (x >> 1) * BN, lt);
+                    const uint32_t own = __reduce_max_sync(0xffffffffu, tile.most());
+                    if (lane == 0) sm.most[kv & 1][warp - LOAD_WARP] = own;
                     if (named_sync_or(1, 128, !ok || failed)) {
                         failed = true;
                         break;
                     }
-                    tile.write(sm.kv[st], lt);
+                    const uint32_t* w = sm.most[kv & 1];
+                    float unit = unit_2_14(max(max(w[0], w[1]), max(w[2], w[3])));
+                    if (x & 1) unit = unit_v = x == 1 || unit > unit_v ? 4.f * unit : unit_v;
+                    if (lt == 0) sm.unit_kv[kv % UNITS] = unit;
+                    tile.write(sm.kv[st], inverse_of_power(unit), lt);
                     fence_async_smem();
                     mbar_arrive(&sm.kv_full[st]);
                 }
@@ -1071,12 +1142,15 @@ __global__ void __launch_bounds__(128) packed_join(const __grid_constant__ Param
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int q = j.first_cta; q <= c; ++q) {
         const long slot = 2L * q + (q == j.first_cta ? 1 : 0);
-        const float2 ml = p.part_ml[slot * ITEM_ROWS + r];
-        if (ml.y == 0.f) continue;  // the row saw none of the part's keys
-        const float top = fmaxf(big, ml.x);
-        const float keep = ex2(big - top), mine = ex2(ml.x - top);
+        const float lse = p.part_lse[slot * ITEM_ROWS + r];
+        if (lse == -INFINITY) continue;  // the row saw none of the part's keys
+        const float top = fmaxf(big, lse);
+        float keep = l * ex2(big - top), mine = ex2(lse - top);
         big = top;
-        l = fmaf(l, keep, ml.y * mine);
+        l = keep + mine;
+        const float inv = 1.f / l;  // normalised at every step: nothing passes the largest |v|
+        keep *= inv;
+        mine *= inv;
         const float4* src = p.part_o + (slot * (D / 4) + w * (E / 4)) * ITEM_ROWS + r;
 #pragma unroll
         for (int e = 0; e < E / 4; ++e) {
@@ -1087,7 +1161,6 @@ __global__ void __launch_bounds__(128) packed_join(const __grid_constant__ Param
             acc[4 * e + 3] = fmaf(acc[4 * e + 3], keep, v.w * mine);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
     const int h = j.hk * p.G + row % p.G;
     const long at = j.q0 + row / p.G;
     T* out = static_cast<T*>(p.a.o) + at * p.a.ld_o + h * D + w * E;
@@ -1095,7 +1168,7 @@ __global__ void __launch_bounds__(128) packed_join(const __grid_constant__ Param
     for (int e = 0; e < E; e += 16 / static_cast<int>(sizeof(T))) {
         Vec16<T> y;
 #pragma unroll
-        for (int i = 0; i < Vec16<T>::N; ++i) y.x[i] = from_f32<T>(acc[e + i] * inv);
+        for (int i = 0; i < Vec16<T>::N; ++i) y.x[i] = from_f32<T>(acc[e + i]);
         *reinterpret_cast<uint4*>(out + e) = y.raw;
     }
     if (w == 0) p.a.lse[static_cast<long>(h) * p.a.Nq + at] = l == 0.f ? -INFINITY : (big + log2f(l)) * kLn2;
@@ -1149,13 +1222,13 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
              head_items * a.Hkv * (static_cast<long>(a.Nk) / C::BN + ITEM_COST + 1) <= INT_MAX;
     const int ctas = p.line || head_items * a.Hkv > num_sms ? num_sms : static_cast<int>(head_items * a.Hkv);
     char* ws = nullptr;
-    const size_t o_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS * D, ml_bytes = sizeof(float2) * 2 * ctas * ITEM_ROWS;
+    const size_t o_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS * D, lse_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS;
     if (p.line) {
-        st.cuda = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), o_bytes + ml_bytes + sizeof(Join) * ctas, pool, stream);
+        st.cuda = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), o_bytes + lse_bytes + sizeof(Join) * ctas, pool, stream);
         if (!st.ok()) return st;
         p.part_o = reinterpret_cast<float4*>(ws);
-        p.part_ml = reinterpret_cast<float2*>(ws + o_bytes);
-        p.joins = reinterpret_cast<Join*>(ws + o_bytes + ml_bytes);
+        p.part_lse = reinterpret_cast<float*>(ws + o_bytes);
+        p.joins = reinterpret_cast<Join*>(ws + o_bytes + lse_bytes);
     }
     st.cuda = launch_pdl(kernel, dim3(ctas), dim3(N_THREADS), smem, stream, p);
     if (st.ok()) ++*launches;

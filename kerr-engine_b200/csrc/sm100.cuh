@@ -526,6 +526,29 @@ __device__ __forceinline__ void split2_x2(float a, float b, uint32_t& hi, uint32
     lo = pack_bf16(ra, rb);
 }
 
+// Two f32 as f16 pairs: x = hi + lo, off by 2^-22 |x| at most where lo is normal
+// (|x| from 2^-3 on), and by 2^-25 below.
+__device__ __forceinline__ void split2_f16(uint64_t ab, uint32_t& hi, uint32_t& lo) {
+    float x, y;
+    f2_unpack(ab, x, y);
+    hi = pack_f16(x, y);
+    asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(hi));
+    f2_unpack(f2_sub(ab, f2_pack(x, y)), x, y);
+    lo = pack_f16(x, y);
+}
+
+// The power of two that numbers whose largest magnitude has the bits `most` are
+// divided by to lie in [2^14, 2^15); one for infinities and NaN.  At least 2^-114.
+__device__ __forceinline__ float unit_2_14(uint32_t most) {
+    const int e = most < 0x7F800000u ? max(static_cast<int>(most >> 23), 27) : 127 + 14;
+    return __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+}
+__device__ __forceinline__ float inverse_of_power(float x) {  // of a power of two in 2^-126 .. 2^126
+    return __uint_as_float((254u << 23) - __float_as_uint(x));
+}
+
 // Byte offset of (row, 16-byte chunk) inside a 128B-swizzled tile of 128-byte rows.
 __device__ __forceinline__ uint32_t sw128(uint32_t row, uint32_t chunk) {
     return (row >> 3) * 1024u + (row & 7u) * 128u + ((chunk ^ (row & 7u)) << 4);

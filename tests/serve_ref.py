@@ -5,15 +5,20 @@ Bounds.  With u = eps/2 of a type (half a step: f32 2^-24, f16 2^-11, bf16
 2^-8), a row's scores s_j, weights p_j (sum one) and A = sum_j p_j |v_j|:
 
 - A score is off by at most D = c_s * |scale| * max_j sum_i |q_i k_ji|, where
-  c_s = 3 * 2^-18 for f32 (products of bf16 hi + lo pairs: each operand is off
-  by 2^-18 of itself and lo * lo, 2^-18, is left out) plus the f32 sums'
+  c_s = 3 * 2^-22 for f32 (products of f16 hi + lo pairs, 11 bits each: each
+  operand is off by 2^-22 of itself and lo * lo, 2^-22, is left out) plus the f32 sums'
   (d + 3) * 2^-24, which stand alone for 16-bit types, whose products are exact.
+  Pairs stand behind a power of two that brings the largest of a row or of some
+  keys to 2^14 or above; below 2^-3 the lo loses up to 2^-25, so an element is off
+  by 2^-39 of the largest besides: a score by |scale| * 2 * d * 2^-39 max|q| max|k|.
 - Weights change by a factor within exp(+-2 D), exp2's own 2^-21 included by
   adding it to D: o moves by at most 2 D A.
 - Weights enter the second product rounded: by u of the type for 16-bit types
   (c_v = u; the unnormalised weights, at most 2^8, lose at most 2^-24 below
   f16's normal range, and there are `keys` of them: keys * 2^-24 * max|v|),
-  by 3 * 2^-18 for f32; its f32 sums and the division add (keys + 8) * 2^-24.
+  by 3 * 2^-22 for f32, where a weight, held times 2^7 and at least one for some key,
+  is off by 2^-32 besides, and v by 2^-37 of the largest (its power of two is kept for
+  keys up to four times the first): (keys * 2^-32 + 2^-37) * max|v|; its f32 sums and the division add (keys + 8) * 2^-24.
 - The output is rounded once: u |o|.
 - lse is off by D, by 2^-21 for the logarithm, and by its rounding, 2^-23 |lse|.
 """
@@ -44,11 +49,14 @@ def attend(q, k, v, seen, scale, dtype):
     o = p @ vz
     A = p @ vz.abs()
     u = U[dtype]
-    c_s = (3 * 2.0 ** -18 if dtype == torch.float32 else 0.0) + (d + 3) * 2.0 ** -24
+    c_s = (3 * 2.0 ** -22 if dtype == torch.float32 else 0.0) + (d + 3) * 2.0 ** -24
     most = torch.where(seen, (qh.abs() @ kh.abs().mT) * abs(scale), 0.0).amax(-1)
     D = c_s * most + 2.0 ** -21
-    c_v = 3 * 2.0 ** -18 if dtype == torch.float32 else u
-    low = 0.0 if dtype == torch.float32 else length * 2.0 ** -24 * vz.abs().amax((1, 2))[:, None, None]
+    if dtype == torch.float32:
+        D = D + abs(scale) * 2 * d * 2.0 ** -39 * qh.abs().amax(-1) * kh.abs().amax((1, 2))[:, None]
+    c_v = 3 * 2.0 ** -22 if dtype == torch.float32 else u
+    low = (length * 2.0 ** -32 + 2.0 ** -37 if dtype == torch.float32 else length * 2.0 ** -24) * \
+        vz.abs().amax((1, 2))[:, None, None]
     bo = A * (2 * D[..., None] + c_v + (length + 8) * 2.0 ** -24) + low + u * o.abs() + 1e-30
     bl = D + 2.0 ** -21 + 2.0 ** -23 * torch.where(some, lse, 0.0).abs()
     return o.transpose(0, 1), lse, bo.transpose(0, 1), bl

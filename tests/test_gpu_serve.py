@@ -105,6 +105,22 @@ def test_packed_running_maximum(ctx, dtype, order):
     check_packed(ctx, q, k, v, [0, n], [0, n], H, H, scale=0.0)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("v_from,v_to", [(-30, 30), (30, -30), (0, 12), (-38, -38), (37, 37)])
+def test_packed_f32_magnitudes(ctx, v_from, v_to, d):
+    # Far powers of ten: v's from the first key to the last, q's and k's by row (their products near one),
+    # one column of each a thousand times the others.
+    gen = torch.Generator().manual_seed(8)
+    n, H = 500, 2
+    q, k, v = (torch.randn(n, H * d, generator=gen) for _ in range(3))
+    v = v.clamp(-3, 3) * torch.logspace(v_from, v_to, n, dtype=torch.float64)[:, None].float()
+    q[:, 3] *= 1e3
+    k[:, 5] *= 1e3
+    v[:, 7] *= 1e3 if v_to < 30 and v_from < 30 else 1e-3
+    up = 10.0 ** (16 * torch.rand(1, generator=gen).item())
+    check_packed(ctx, (q * up).cuda(), (k / up).cuda(), v.cuda(), [0, 200, n], [0, 200, n], H, H)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [32, 128])
 def test_packed_strides_and_padding(ctx, dtype, d):
