@@ -406,16 +406,17 @@ int kattn_block_bwd(kattn_ctx* ctx, kattn_block* blk, const float* dh_out, float
  * rows before cu[0] and behind cu[S] are neither read nor written, so arrays
  * padded to a fixed N (a captured graph) are fine.  Query heads are grouped:
  * query head h uses key head h / (H / Hkv), H a multiple of Hkv.  lse is
- * [H][N].  Lengths, tables and pages live on the device; the calls read them
- * there and never synchronise the host.
+ * [H][N].  Rows times heads, and the positions of a table, are below 2^31 - 256.
+ * Lengths, tables and pages live on the device; the calls read them there and
+ * never synchronise the host.
  *
  * Types.  dtype names the element type of q, k, v and o: scores, softmax
  * statistics and sums are formed in f32, and outputs are rounded once.  Products
  * of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about 1e-6,
  * with 2^-37 of the largest magnitude among a sequence's rows as the least step.
- * Sums of v are formed before they are divided: |v| is to stay below 2^96.  Device pointers
- * are 16-byte aligned and row strides a multiple of 16 bytes; int32 arrays
- * and lse 4-byte, tree 8-byte aligned.  d is 32, 64 or 128.
+ * Sums of v are formed before they are divided: |v| is to stay below 2^96.
+ * Device pointers are 16-byte aligned and row strides a multiple of 16 bytes;
+ * int32 arrays and lse 4-byte, tree 8-byte aligned.  d is 32, 64 or 128.
  *
  * A row that sees nothing has o = 0 and lse = -inf.  A NaN or an infinity in
  * a sequence's rows reaches the outputs of that sequence only. */

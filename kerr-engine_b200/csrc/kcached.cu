@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 prefetch_tensormap(&p.tk);
                 prefetch_tensormap(&p.tv);
             }
-            const int capacity = static_cast<int>(min(static_cast<long>(b.max_pages) << p.page_shift, 0x7FFFFFC0L));
+            const int capacity = b.max_pages << p.page_shift;
             Line<MR> line{a, p.G, lane, capacity};
             const int frag_shift = min(p.page_shift, 7), frag = 1 << frag_shift;  // a stretch of a page that a copy takes
             bool more = line.start(blockIdx.x, gridDim.x);

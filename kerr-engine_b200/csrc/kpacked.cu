@@ -171,7 +171,12 @@ struct Params {
     float* part_lse;  // [2 * CTAs][256 rows]: log2 of the rows' sums
     Join* joins;      // [CTAs]
     // x / G for x below 2^32 / G (the product is off by less than x G / 2^32).
-    __device__ __forceinline__ int div(int x) const { return G == 1 ? x : static_cast<int>(__umulhi(x, inv_g)); }
+    // x / G: the product is at most one too large, and is from x = 2^32 / G on.
+    __device__ __forceinline__ int div(int x) const {
+        if (G == 1) return x;
+        const uint32_t y = __umulhi(x, inv_g);
+        return static_cast<int>(y - (y * G > static_cast<uint32_t>(x) ? 1u : 0u));
+    }
 };
 
 // ---------------------------------------------------------------- items
@@ -219,13 +224,17 @@ struct ItemFinder {
     }
     __device__ __forceinline__ void start() {
         int nk = 0;
+        long items = 0;
 #pragma unroll 1
         for (int s = lane; s < a.S; s += 32) {
-            const int2 k = seq_rows(a.cu_k, s, a.Nk);
+            const int2 q = seq_rows(a.cu_q, s, a.Nq), k = seq_rows(a.cu_k, s, a.Nk);
             nk = max(nk, k.y - k.x);
+            items += static_cast<long>(items_at_least<BN>(q.y - q.x, k.y - k.x, G, a.causal, 0)) * a.Hkv;
         }
         level = (__reduce_max_sync(0xffffffffu, nk) + BN - 1) / BN;
-        total = count(0);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
+        total = items <= INT_MAX ? static_cast<int>(items) : 0;  // (ascending offsets make no more)
     }
     // The k-th item (k not below an earlier call's).
     __device__ __forceinline__ Item find(int k) {
@@ -336,7 +345,7 @@ __device__ __forceinline__ void plan_line(S& sm, const Params& p, int tid) {
     }
     int sum = block_scan(own, pl.warp_sum, tid);
     if (tid < a.S) pl.item0[tid] = sum - own;
-    if (tid == N_THREADS - 1) sm.head_items = sum;
+    if (tid == N_THREADS - 1) sm.head_items = min(sum, PLAN);  // (ascending offsets make no more)
     __syncthreads();
     const int items = sm.head_items;
     own = 0;
@@ -1219,7 +1228,7 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
     // Each sequence ends at most one item that is not full.
     const long head_items = static_cast<long>(a.Nq) * p.G / ITEM_ROWS + a.S;
     p.line = head_items <= PLAN && head_items * a.Hkv < LINE_ITEMS * num_sms &&
-             head_items * a.Hkv * (static_cast<long>(a.Nk) / C::BN + ITEM_COST + 1) <= INT_MAX;
+             PLAN * static_cast<long>(a.Hkv) * (a.Nk / C::BN + ITEM_COST + 1) <= INT_MAX;
     const int ctas = p.line || head_items * a.Hkv > num_sms ? num_sms : static_cast<int>(head_items * a.Hkv);
     char* ws = nullptr;
     const size_t o_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS * D, lse_bytes = sizeof(float) * 2 * ctas * ITEM_ROWS;

@@ -56,6 +56,8 @@ int check_array(const char* name, const void* p, int align) {
 
 int check_counts(int S, int N) {
     if (S < 0 || N < 0) return fail(KATTN_ERR_INVALID_ARGUMENT, "negative size (S=%d N=%d)", S, N);
+    if (S > INT_MAX - 256 || N > INT_MAX - 256)
+        return fail(KATTN_ERR_INVALID_ARGUMENT, "problem too large (S=%d N=%d)", S, N);
     return KATTN_OK;
 }
 
@@ -78,11 +80,13 @@ int check_cache(const kattn_kv_cache* c) {
     return KATTN_OK;
 }
 
-int check_batch(const int* cu, const int* kv_len, const int* table, long ld_table, int max_pages) {
+int check_batch(const int* cu, const int* kv_len, const int* table, long ld_table, int max_pages, int page_size) {
     KATTN_TRY(check_array("cu", cu, 4));
     KATTN_TRY(check_array("kv_len", kv_len, 4));
     if (max_pages < 0 || ld_table < max_pages)
         return fail(KATTN_ERR_INVALID_ARGUMENT, "table row stride %ld < max_pages %d", ld_table, max_pages);
+    if (static_cast<long>(max_pages) * page_size > INT_MAX - 256)
+        return fail(KATTN_ERR_INVALID_ARGUMENT, "max_pages * page_size too large (%d, %d)", max_pages, page_size);
     if (max_pages > 0) KATTN_TRY(check_array("table", table, 4));
     return KATTN_OK;
 }
@@ -103,7 +107,7 @@ int cache_rows_checks(const kattn_ctx* ctx, const kattn_kv_cache* cache, int dty
     const long cols = static_cast<long>(cache->n_kv_head) * cache->d;
     KATTN_TRY(check_rows("k", k, ld_kv, cols, dtype));
     KATTN_TRY(check_rows("v", v, ld_kv, cols, dtype));
-    return check_batch(cu, kv_len, table, ld_table, max_pages);
+    return check_batch(cu, kv_len, table, ld_table, max_pages, cache->page_size);
 }
 
 }  // namespace
@@ -120,7 +124,7 @@ int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const 
     KATTN_TRY(check_heads(H, Hkv, d));
     KATTN_TRY(check_counts(S, Nq));
     if (Nk < 0) return fail(KATTN_ERR_INVALID_ARGUMENT, "negative size (Nk=%d)", Nk);
-    if (static_cast<long>(Nq) * H > INT_MAX || Nk > INT_MAX - 256 || static_cast<long>(S) * Hkv > INT_MAX / 2)
+    if (static_cast<long>(Nq) * H > INT_MAX - 256 || Nk > INT_MAX - 256 || static_cast<long>(S) * Hkv > INT_MAX / 2)
         return fail(KATTN_ERR_INVALID_ARGUMENT, "problem too large (Nq=%d H=%d Nk=%d S=%d)", Nq, H, Nk, S);
     if (!std::isfinite(scale)) return fail(KATTN_ERR_INVALID_ARGUMENT, "scale is not finite");
     if (causal != 0 && causal != 1) return fail(KATTN_ERR_INVALID_ARGUMENT, "causal must be 0 or 1");
@@ -183,12 +187,14 @@ int kattn_fwd_cached(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, con
     KATTN_TRY(check_dtype(dtype));
     KATTN_TRY(check_heads(H, cache->n_kv_head, cache->d));
     KATTN_TRY(check_counts(S, N));
+    if (static_cast<long>(N) * H > INT_MAX - 256)
+        return fail(KATTN_ERR_INVALID_ARGUMENT, "problem too large (N=%d H=%d)", N, H);
     if (!std::isfinite(scale)) return fail(KATTN_ERR_INVALID_ARGUMENT, "scale is not finite");
     if (S == 0 || N == 0) return ok_with_launches(0);
     KATTN_TRY(check_rows("q", q, ld_q, static_cast<long>(H) * cache->d, dtype));
     KATTN_TRY(check_rows("o", o, ld_o, static_cast<long>(H) * cache->d, dtype));
     KATTN_TRY(check_array("lse", lse, 4));
-    KATTN_TRY(check_batch(cu, kv_len, table, ld_table, max_pages));
+    KATTN_TRY(check_batch(cu, kv_len, table, ld_table, max_pages, cache->page_size));
     if (tree) KATTN_TRY(check_array("tree", tree, 8));
     DeviceScope scope(ctx->device);
     if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");

@@ -172,6 +172,33 @@ def test_packed_broken_offsets_stay_inside(ctx):
     assert (guard[:20] == 3).all() and (guard[20 + N:] == 3).all()
 
 
+@pytest.mark.parametrize("sequences", [200, 3000])
+def test_packed_overlapping_offsets_stay_inside(ctx, sequences):
+    # Offsets that rise and fall: every other sequence owns all rows, far more items than rows make.
+    H, Hkv, d, N = 4, 1, 64, 1000
+    q, k = torch.randn(N, H * d, device="cuda"), torch.randn(N, Hkv * d, device="cuda")
+    guard = torch.full((N + 40, H * d), 3.0, device="cuda")
+    o, lse = guard[20:20 + N], torch.zeros(H, N, device="cuda")
+    cu = ints([0, N] * sequences)
+    kerr_attn.fwd_packed(ctx, q, k, k, o, lse, cu, cu, H, Hkv)
+    torch.cuda.synchronize()
+    assert (guard[:20] == 3).all() and (guard[20 + N:] == 3).all()
+
+
+def test_packed_wide_group_long(ctx):
+    # Rows times the group's heads past 2^32 / group: every row sees the one key.
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    H, d, n = 512, 32, 18000
+    q = torch.randn(n, H * d, device="cuda", generator=gen).bfloat16()
+    k, v = (torch.randn(1, d, device="cuda", generator=gen).bfloat16() for _ in range(2))
+    o, lse = torch.full_like(q, 7.0), torch.zeros(H, n, device="cuda")
+    kerr_attn.fwd_packed(ctx, q, k, v, o, lse, ints([0, n]), ints([0, 1]), H, 1, causal=False, scale=1.0)
+    assert torch.equal(o.view(n, H, d), v.expand(n, H, d))
+    exact = q.view(n, H, d).double() @ k[0].double()
+    most = q.view(n, H, d).double().abs() @ k[0].double().abs()
+    assert ((lse.T - exact).abs() <= (d + 3) * 2.0 ** -24 * most + 2.0 ** -20 + 2.0 ** -22 * exact.abs()).all()
+
+
 def test_packed_far_rows(ctx):
     # Rows further apart than 2^31 elements.
     gen = torch.Generator().manual_seed(6)

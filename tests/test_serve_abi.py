@@ -47,6 +47,7 @@ def test_fwd_packed_refusals(L):
     assert call(ldq=516) == MISALIGNED and call(ldk=132) == MISALIGNED and call(ldo=514) == MISALIGNED
     assert call(dtype=0, ldq=518) == MISALIGNED
     assert call(ldq=1 << 40) == INVALID
+    assert call(Nq=1 << 28) == INVALID and call(Nk=(1 << 31) - 1) == INVALID
     for none in (dict(S=0), dict(Nq=0)):
         assert call(q=None, k=None, v=None, o=None, lse=None, cu_q=None, cu_k=None, **none) == 0
         assert kerr_attn.last_launch_count() == 0
@@ -77,6 +78,7 @@ def test_cache_rows_refusals(L, what):
     assert call(S=-1) == INVALID and call(N=-1) == INVALID
     assert call(ld=120) == INVALID and call(ld=132) == MISALIGNED
     assert call(ldt=6) == INVALID and call(max_pages=-1) == INVALID
+    assert call(ldt=1 << 27, max_pages=1 << 27) == INVALID and call(N=(1 << 31) - 1) == INVALID
     for name in ("k", "v", "cu", "kv_len", "pages"):
         assert call(**{name: None}) == INVALID, name
         assert call(**{name: 0x9002}) == MISALIGNED, name
@@ -98,7 +100,8 @@ def test_fwd_cached_refusals(L):
     assert call(S=-1) == INVALID and call(N=-1) == INVALID
     assert call(scale=math.inf) == INVALID
     assert call(ldq=500) == INVALID and call(ldo=516) == MISALIGNED
-    assert call(ldt=3) == INVALID
+    assert call(ldt=3) == INVALID and call(ldt=1 << 27, max_pages=1 << 27) == INVALID
+    assert call(N=1 << 28) == INVALID
     assert call(tree=0x7004) == MISALIGNED
     for name in ("q", "o", "lse", "cu", "kv_len", "pages"):
         assert call(**{name: None}) == INVALID, name
