@@ -13,6 +13,10 @@
 // an infinity is larger than a number; 16-bit ones two at a time), and a lane's place is kept by
 // additions.  A block streams groups of tokens, two 16-byte pieces of a row to a lane; its
 // ninth warp looks up the next group's sequences and pages (a chain of loads) meanwhile.
+//
+// Measured: 97k bf16 tokens, 8 heads of 128, written to int8 codes and read back, 999 MB: 235 us,
+// 5.1 TB/s of the codes and rows that both calls move (343 us with one piece to a lane and the
+// lookups in line); 18k f32 positions of 12 heads of 64 read back, 106 MB: 23 us, 4.6 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -223,70 +227,58 @@ template <class T, int FORMAT>
 __global__ void __launch_bounds__(kBlock, kBlocksPerSm) cache_read_rows(CacheArgs a, T* __restrict__ k, T* __restrict__ v, long ld,
                                                           int page_shift, int tokens) {
     constexpr int E = Vec16<T>::N;
-    constexpr int U = 1;  // rows of a lane at a time
     pdl_enter();
     const int d = a.c.d, lanes = d / (2 * E), heads = a.c.n_kv_head;
     const int c = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = kThreads / lanes;
     for_groups(a, page_shift, tokens, [&](int t0, int n, const long* place) {
         Walk w(first, step, heads);
-        for (int r = first; r < n * heads * 2; r += U * step) {
-            uint32_t code[U][2][E / 4];
-            float scale[U];
-            uint4* to[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u, w.next()) {
-                const int token = w.tk >> 1;
-                const bool is_v = w.tk & 1;
-                const long at = token < n ? place[token] : kNoRow;
-                to[u] = at != kNoRow ? reinterpret_cast<uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld +
-                                                                w.head * d) + c
-                                     : nullptr;
-                scale[u] = 0.f;
-#pragma unroll
-                for (int i = 0; i < E / 4; ++i) code[u][0][i] = code[u][1][i] = 0;
-                if (at >= 0) {
-                    const long row = at + (static_cast<long>(w.head) << page_shift);
-                    const uint8_t* from = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if constexpr (E == 4) {
-                            code[u][h][0] = __ldcs(reinterpret_cast<const uint32_t*>(from + h * lanes * E));
-                        } else {
-                            const uint2 y = __ldcs(reinterpret_cast<const uint2*>(from + h * lanes * E));
-                            code[u][h][0] = y.x;
-                            code[u][h][1] = y.y;
-                        }
-                    }
-                    scale[u] = __ldg((is_v ? a.c.v_scale : a.c.k_scale) + row);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (!to[u]) continue;
+        for (int r = first; r < n * heads * 2; r += step, w.next()) {
+            const int token = w.tk >> 1;
+            const bool is_v = w.tk & 1;
+            const long at = token < n ? place[token] : kNoRow;
+            if (at == kNoRow) continue;
+            uint4* to = reinterpret_cast<uint4*>((is_v ? v : k) + static_cast<long>(t0 + token) * ld + w.head * d) + c;
+            float scale = 0.f;
+            uint32_t code[2][E / 4] = {};
+            if (at >= 0) {
+                const long row = at + (static_cast<long>(w.head) << page_shift);
+                const uint8_t* from = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + row * d + c * E;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float f[E];
-#pragma unroll
-                    for (int i = 0; i < E / 4; ++i) decode4<FORMAT>(code[u][h][i], scale[u], f + 4 * i);
-                    uint4 y;
-                    if constexpr (sizeof(T) == 4) {
-                        y = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                       __float_as_uint(f[3]));
-                    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-                        y = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
-                                       pack_bf16(f[6], f[7]));
+                    if constexpr (E == 4) {
+                        code[h][0] = __ldcs(reinterpret_cast<const uint32_t*>(from + h * lanes * E));
                     } else {
-                        y = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]),
-                                       pack_f16(f[6], f[7]));
+                        const uint2 y = __ldcs(reinterpret_cast<const uint2*>(from + h * lanes * E));
+                        code[h][0] = y.x;
+                        code[h][1] = y.y;
                     }
-                    __stcs(&to[u][h * lanes], y);
                 }
+                scale = __ldg((is_v ? a.c.v_scale : a.c.k_scale) + row);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float f[E];
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i) decode4<FORMAT>(code[h][i], scale, f + 4 * i);
+                uint4 y;
+                if constexpr (sizeof(T) == 4) {
+                    y = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                   __float_as_uint(f[3]));
+                } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                    y = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
+                                   pack_bf16(f[6], f[7]));
+                } else {
+                    y = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]),
+                                   pack_f16(f[6], f[7]));
+                }
+                __stcs(&to[h * lanes], y);
             }
         }
     });
 }
 
-// Tokens of a group: up to 16, fewer where they would leave SMs without one; the
+// Tokens of a group: up to 16, fewer where they would leave SMs without one (64 tokens of a
+// decoding step: a group each, 3.5 us a call; in groups of 16 only four blocks would work); the
 // grid is as many blocks as fit at once.
 int group_tokens(int N, int num_sms) {
     int t = 1;

@@ -12,9 +12,14 @@
 // a work item is 256 of them: two tiles of 128, which read the same K and V
 // tiles.  A group of few tokens then still fills its tile.
 //
-// Work.  With many items to a CTA, each takes whole ones, longest first.  A
-// small problem's items are one line of key tiles cut into equal parts, one a CTA
-// (few long sequences then still fill the GPU); packed_join adds the parts of cut items.
+// Work.  Where enough items share the GPU, each CTA takes whole ones, longest first.  A few long
+// ones are a line of key tiles cut into equal parts, one a CTA, and packed_join adds the
+// parts of cut items; line_pays() has the rule and what both measured.
+//
+// Bounds.  Long prompts: the tensor core's rate, shared with the exponentials (three bf16 prompts of
+// 1500 .. 8192, 32 heads of 128: 574 us, 1110 TFLOP/s).  f32: three products of each, whose
+// operands shared memory feeds, 3300 clocks a step.  Short prompts: the chain from launch to first copy
+// to store (one f32 prompt of 256, 12 heads: 19 us; 32 bf16 prompts of 9 .. 512, 20 heads on 4: 27 us).
 //
 // Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
 // one thread a row.  8-11: Q into shared memory (and, for f32, K and V split
@@ -32,12 +37,13 @@
 // ones as f16 pairs (22 bits), hi*hi + hi*lo + lo*hi, after powers of two have brought
 // them near 2^14: one a row of Q, one a tile of K, one for the V tiles of an item (it
 // rises when one needs it, and O follows).  They go back in with the exponent's factor
-// and the output.  bf16 pairs need no powers and took 84 us where this takes 93 (chunks
+// and the output.  bf16 pairs need no powers and took 84 us where this takes 94 (chunks
 // over cached contexts, f32), but are off by 6e-6; these by 3e-7 to 9e-7, as an f32 product is.
 //
 // Weights are 2^(c s - c mu), c = scale log2(e), with mu raised only when a
 // tile's maximum passes it by more than 2^8 (then O and the sum are scaled): weights
 // stay below 2^8, which f16 holds, and O is almost never read back.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 
@@ -293,11 +299,23 @@ struct ItemFinder {
     }
 };
 
-// Small problems: all items are one line of steps, ITEM_COST more for
-// each (its rows, its output), cut into equal parts of at least MIN_PART.  A
-// border moves to an item's edge that is near.
+// All items as one line of steps, ITEM_COST more for each (its rows, its output), cut
+// into equal parts of at least MIN_PART.  A border moves to an item's edge that is near.
 constexpr int ITEM_COST = 3, MIN_PART = 5;
-constexpr long LINE_ITEMS = 6;  // items to a CTA below which a problem is small
+
+// Whether the line pays, by the lengths that the host knows, in steps of 128 keys.  Whole items
+// end with the longest: an average prompt (a longer one has more items too, which hide it) behind
+// three times the average context, as contexts differ.  Parts end with the mean, but plan
+// and join cost what 5 steps do.  Dealt whole and in parts, us: one bf16 prompt of 1024 and of
+// 2048, 12 heads of 64, 20.6 and 23.4, 34.3 and 29.3; 16 of 512, 12 heads on 4, 29.2 and 37.5; 8 f32
+// chunks of 100 .. 1000 behind up to 3096 positions 112 and 94; three bf16 prompts of 1500 ..
+// 8192, 32 heads of 128 on 8, 576 and 644.
+inline bool line_pays(const PackedArgs& a, long items, int num_sms) {
+    const double nk = static_cast<double>(a.Nk) / a.S, nq = std::min(static_cast<double>(a.Nq) / a.S, nk);
+    const double mean = items / static_cast<double>(num_sms) * (nk - (a.causal ? nq / 2 : 0)) / 128;
+    const double longest = std::min(nq + 3 * (nk - nq), static_cast<double>(a.Nk)) / 128;
+    return longest - std::max<double>(mean, MIN_PART) > 5;
+}
 
 template <int BN>
 __device__ __forceinline__ int item_cost(int2 seq, int G, int causal, int item) {
@@ -1227,7 +1245,7 @@ ProjStatus launch(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStre
     }
     // Each sequence ends at most one item that is not full.
     const long head_items = static_cast<long>(a.Nq) * p.G / ITEM_ROWS + a.S;
-    p.line = head_items <= PLAN && head_items * a.Hkv < LINE_ITEMS * num_sms &&
+    p.line = head_items <= PLAN && line_pays(a, head_items * a.Hkv, num_sms) &&
              PLAN * static_cast<long>(a.Hkv) * (a.Nk / C::BN + ITEM_COST + 1) <= INT_MAX;
     const int ctas = p.line || head_items * a.Hkv > num_sms ? num_sms : static_cast<int>(head_items * a.Hkv);
     char* ws = nullptr;

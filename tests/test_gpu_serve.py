@@ -52,7 +52,15 @@ def check_packed(ctx, q, k, v, cu_q, cu_k, H, Hkv, causal=True, scale=None):
     want, wl, bo, bl = serve_ref.packed(q, k, v, cu_q, cu_k, H, Hkv, causal, sc)
     serve_ref.check(o, want, bo, "o")
     serve_ref.check(lse, wl, bl, "lse")
+    # Rows of keys behind the last sequence's make the work look long: it is cut into parts.
+    o2, lse2 = run_packed(ctx, q, *(long_rows(x, len(cu_q) - 1) for x in (k, v)), cu_q, cu_k, H, Hkv, causal, scale)
+    serve_ref.check(o2, want, bo, "o in parts")
+    serve_ref.check(lse2, wl, bl, "lse in parts")
     return o, lse
+
+
+def long_rows(x, sequences):
+    return torch.cat([x, torch.full((4000 * sequences, x.shape[1]), float("nan"), dtype=x.dtype, device="cuda")])
 
 
 # Query rows, key rows (None: the same), query and key heads of each sequence.
@@ -65,6 +73,7 @@ PACKED = {
     "chunks": ([3, 128, 17, 1], [300, 129, 17, 513], 4, 2),
     "fewer_keys": ([40, 200, 9], [10, 0, 9], 2, 1),
     "longer": ([700, 1030], None, 2, 1),
+    "far_context": ([3, 200, 0, 40], [2000, 3500, 300, 2600], 4, 2),
 }
 
 
@@ -172,11 +181,11 @@ def test_packed_broken_offsets_stay_inside(ctx):
     assert (guard[:20] == 3).all() and (guard[20 + N:] == 3).all()
 
 
-@pytest.mark.parametrize("sequences", [200, 3000])
-def test_packed_overlapping_offsets_stay_inside(ctx, sequences):
+@pytest.mark.parametrize("sequences,keys", [(200, 1000), (200, 400000), (3000, 1000)])
+def test_packed_overlapping_offsets_stay_inside(ctx, sequences, keys):
     # Offsets that rise and fall: every other sequence owns all rows, far more items than rows make.
     H, Hkv, d, N = 4, 1, 64, 1000
-    q, k = torch.randn(N, H * d, device="cuda"), torch.randn(N, Hkv * d, device="cuda")
+    q, k = torch.randn(N, H * d, device="cuda"), torch.randn(keys, Hkv * d, device="cuda")
     guard = torch.full((N + 40, H * d), 3.0, device="cuda")
     o, lse = guard[20:20 + N], torch.zeros(H, N, device="cuda")
     cu = ints([0, N] * sequences)
@@ -562,7 +571,9 @@ def test_captured_steps_follow_their_lengths(ctx):
     H, Hkv, d, page, S, N = 4, 2, 64, 16, 3, 12
     cache, table = make_cache([400, 400, 400], page, Hkv, d, 0, seed=12)
     gen = torch.Generator().manual_seed(23)
-    q, k, v = randn(gen, N, H * d), randn(gen, N, Hkv * d), randn(gen, N, Hkv * d)
+    q = randn(gen, N, H * d)
+    long_k, long_v = (long_rows(randn(gen, N, Hkv * d), S) for _ in range(2))  # packed work in parts: a workspace
+    k, v = long_k[:N], long_v[:N]
     cu, kv_len = ints([0, 1, 2, 3]), ints([1, 1, 1])
     outs = [(torch.zeros_like(q), torch.zeros(H, N, device="cuda")) for _ in range(2)]
     packed = (torch.zeros_like(q), torch.zeros(H, N, device="cuda"))
@@ -574,7 +585,7 @@ def test_captured_steps_follow_their_lengths(ctx):
         with torch.cuda.graph(g, stream=side):
             kerr_attn.cache_append(ctx, cache, k, v, cu, kv_len, table)
             kerr_attn.fwd_cached(ctx, cache, q, o, lse, cu, kv_len, table, H)
-            kerr_attn.fwd_packed(ctx, q, k, v, *packed, cu, cu, H, Hkv)
+            kerr_attn.fwd_packed(ctx, q, long_k, long_v, *packed, cu, cu, H, Hkv)
         graphs.append(g)
     length = [0, 0, 0]
     for turn, new in enumerate(([4, 2, 3], [1, 1, 1], [5, 0, 7], [2, 2, 2], [1, 1, 1])):
@@ -608,9 +619,9 @@ def test_two_streams_at_once(ctx):
         cache, table = make_cache(kv_len, page, Hkv, d, i, seed=13 + i)
         fill(ctx, cache, table, kv_len, torch.bfloat16, seed=24 + i)
         q = randn(torch.Generator().manual_seed(26 + i), 4, H * d, dtype=torch.bfloat16)
-        k = randn(torch.Generator().manual_seed(28 + i), 500, Hkv * d)
+        k = randn(torch.Generator().manual_seed(28 + i), 3000, Hkv * d)
         jobs.append((cache, table, kv_len, q, k, run_cached(ctx, cache, q, [3, 1], kv_len, table, H),
-                     run_packed(ctx, torch.cat([k] * 4, 1), k, k, [0, 500], [0, 500], H, Hkv)))
+                     run_packed(ctx, torch.cat([k[:500]] * 4, 1), k, k, [0, 500], [0, 3000], H, Hkv)))
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     got = [[], []]
@@ -619,7 +630,7 @@ def test_two_streams_at_once(ctx):
             cache, table, kv_len, q, k, _, _ = jobs[i]
             with torch.cuda.stream(s):
                 got[i].append((run_cached(ctx, cache, q, [3, 1], kv_len, table, H),
-                               run_packed(ctx, torch.cat([k] * 4, 1), k, k, [0, 500], [0, 500], H, Hkv)))
+                               run_packed(ctx, torch.cat([k[:500]] * 4, 1), k, k, [0, 500], [0, 3000], H, Hkv)))
     torch.cuda.synchronize()
     for i in range(2):
         for a, b in got[i]:
