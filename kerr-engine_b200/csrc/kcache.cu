@@ -14,8 +14,8 @@
 // additions.  A block streams groups of tokens, two 16-byte pieces of a row to a lane; its
 // ninth warp looks up the next group's sequences and pages (a chain of loads) meanwhile.
 //
-// Measured: 97k bf16 tokens, 8 heads of 128, written to int8 codes and read back, 999 MB: 235 us,
-// 5.1 TB/s of the codes and rows that both calls move (343 us with one piece to a lane and the
+// Measured: 97k bf16 tokens, 8 heads of 128, written to int8 codes and read back, 999 MB: 230 us,
+// 4.3 TB/s, 5.2 with the codes counted as written and as read (343 us with one piece to a lane and the
 // lookups in line); 18k f32 positions of 12 heads of 64 read back, 106 MB: 23 us, 4.6 TB/s.
 #include <algorithm>
 #include <type_traits>

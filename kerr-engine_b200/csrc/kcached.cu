@@ -10,8 +10,8 @@
 // so the work is to keep enough copies in flight and to turn codes into
 // MMA operands with few instructions.  64 bf16 sequences' one token over up to 8191
 // positions, 8 key heads of 128, int8 codes, 347 MB: 86 us, 4.0 TB/s.  With more rows
-// the products' instructions bound it: trees of 8 tokens, 32 rows a key head, over
-// 2 x 131k positions, 370 MB of e4m3: 142 us, 240 TFLOP/s.
+// the products' instructions bound it: trees of 8 tokens, 32 rows a key head, of two
+// sequences of up to 131k positions, 370 MB of e4m3: 143 us, 160 TFLOP/s.
 //
 // Rows.  The G query heads of a key head share its positions: a sequence's n
 // tokens are n * G rows, in row tiles of 8 * NB.  Positions are the m of

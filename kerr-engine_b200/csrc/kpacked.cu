@@ -17,7 +17,7 @@
 // parts of cut items; line_pays() has the rule and what both measured.
 //
 // Bounds.  Long prompts: the tensor core's rate, shared with the exponentials (three bf16 prompts of
-// 1500 .. 8192, 32 heads of 128: 574 us, 1110 TFLOP/s).  f32: three products of each, whose
+// 1500 .. 8192, 32 heads of 128: 570 us, 1130 TFLOP/s; 660 us, 980 TFLOP/s from a cold L2).  f32: three products of each, whose
 // operands shared memory feeds, 3300 clocks a step.  Short prompts: the chain from launch to first copy
 // to store (one f32 prompt of 256, 12 heads: 19 us; 32 bf16 prompts of 9 .. 512, 20 heads on 4: 27 us).
 //
