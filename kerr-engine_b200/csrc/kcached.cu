@@ -74,9 +74,15 @@ struct Params {
     CUtensorMap tk, tv;
     CachedArgs a;
     int page_shift, G;
+    uint32_t inv_g;  // (2^32 - 1) / G
     float* part_o;   // [2 * CTAs][rows][D]: a CTA's part that began before it (0) or begins in it (1)
     float2* part_ml; // [2 * CTAs][rows]
     Join* joins;     // [CTAs]
+    // x / G: the product is at most one too small.
+    __device__ __forceinline__ int div(int x) const {
+        const int y = static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv_g));
+        return y + (x - y * G >= G ? 1 : 0);
+    }
 };
 
 template <int D, int NB, bool SPLIT>
@@ -303,15 +309,34 @@ struct Line {
 };
 
 // ---------------------------------------------------------------- rows
-// Four neighbouring elements of q (16-byte rows, so 8-byte pieces are aligned).
-__device__ __forceinline__ float4 load_q4(const CachedArgs& a, long i) {
-    if (a.dtype == KATTN_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + i));
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + i));
-    if (a.dtype == KATTN_BF16)
-        return make_float4(bf16_lo_f(w.x), bf16_hi_f(w.x), bf16_lo_f(w.y), bf16_hi_f(w.y));
+// Four neighbouring elements of q, as they lie (16-byte rows, so 8-byte pieces are aligned).
+__device__ __forceinline__ float4 widened(const uint4& w, int) {
+    return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+}
+__device__ __forceinline__ float4 widened(const uint2& w, int dtype) {
+    if (dtype == KATTN_BF16) return make_float4(bf16_lo_f(w.x), bf16_hi_f(w.x), bf16_lo_f(w.y), bf16_hi_f(w.y));
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
     const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
     return make_float4(x.x, x.y, y.x, y.y);
+}
+
+// The largest magnitude (a NaN or an infinity above all).
+template <int N>
+__device__ __forceinline__ float largest(const uint4 (&w)[N], int) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        m = max(m, max(max(w[k].x & 0x7FFFFFFFu, w[k].y & 0x7FFFFFFFu), max(w[k].z & 0x7FFFFFFFu, w[k].w & 0x7FFFFFFFu)));
+    return __uint_as_float(min(m, 0x7F800000u));
+}
+template <int N>
+__device__ __forceinline__ float largest(const uint2 (&w)[N], int dtype) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) m = __vmaxu2(m, __vmaxu2(w[k].x & 0x7FFF7FFFu, w[k].y & 0x7FFF7FFFu));
+    m = max(m & 0xFFFFu, m >> 16);
+    if (dtype == KATTN_BF16) return __uint_as_float(min(m << 16, 0x7F800000u));
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(min(m, 0x7C00u))));
 }
 
 // N (a multiple of 4) neighbouring outputs, rounded once.
@@ -458,33 +483,32 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
             }
         } else if (warp >= Q_WARP) {
             // -------------------------------------------------------- q
+            using Raw = std::conditional_t<SPLIT, uint4, uint2>;  // four elements
+            using Element = std::conditional_t<SPLIT, uint32_t, uint16_t>;
             // Operand B, row 8 nb + g: k slots (2t, 2t+1) and (2t+8, 2t+9) of step k are four neighbouring columns.
             for (int i = 0; next_piece(i); ++i) {
                 const int slot = i % C::Q_SLOTS, use = i / C::Q_SLOTS;
                 // The rows' lines start on their way before they are needed one by one.
                 for (int r = 8 * (warp - Q_WARP) + g; r < piece->rows; r += 8 * Q_WARPS) {
-                    const int row = piece->row0 + r;
-                    const long at = static_cast<long>(piece->q0 + row / p.G) * a.ld_q + (piece->hk * p.G + row % p.G) * D;
-                    const int size = a.dtype == KATTN_F32 ? 4 : 2;
+                    const int row = piece->row0 + r, token = p.div(row);
+                    const long at = static_cast<long>(piece->q0 + token) * a.ld_q + (piece->hk * p.G + row - token * p.G) * D;
+                    const int size = SPLIT ? 4 : 2;
                     if (t * 128 < D * size)
                         asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(a.q) + at * size + t * 128));
                 }
                 if (use > 0 && !await(&sm.q_empty[slot], (use - 1) & 1)) return;
 #pragma unroll 1
                 for (int nb = warp - Q_WARP; nb < NB; nb += Q_WARPS) {
-                    const int r = 8 * nb + g, row = piece->row0 + r;
+                    const int r = 8 * nb + g, row = piece->row0 + r, token = p.div(row);
                     const bool in = r < piece->rows;
-                    const long at = static_cast<long>(piece->q0 + row / p.G) * a.ld_q + (piece->hk * p.G + row % p.G) * D;
-                    auto four = [&](int k) {
-                        return in ? load_q4(a, at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4)))
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-                    };
-                    float most = 0.f;
+                    const long at = static_cast<long>(piece->q0 + token) * a.ld_q + (piece->hk * p.G + row - token * p.G) * D;
+                    Raw w[KS];
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
-                        const float4 w = four(k);
-                        most = fmaxf(most, fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))));
+                        const long i = at + 4 * CH * (k / (CH / 4)) + CH * t + 4 * (k % (CH / 4));
+                        w[k] = in ? __ldg(reinterpret_cast<const Raw*>(static_cast<const Element*>(a.q) + i)) : Raw{};
                     }
+                    float most = largest(w, a.dtype);
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                     // The row times 2^(13 - e), e the exponent of its largest element.
@@ -492,10 +516,10 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                     const float up = __uint_as_float(static_cast<uint32_t>(127 + min(13 - e, 127)) << 23);
                     const float down = __uint_as_float(static_cast<uint32_t>(127 + max(e - 13, -126)) << 23);
                     if (t == 0) sm.f[slot][r] = down * (a.scale * kLog2e);
-#pragma unroll 4
+#pragma unroll
                     for (int k = 0; k < KS; ++k) {
-                        const float4 w = four(k);
-                        const float4 v = make_float4(w.x * up, w.y * up, w.z * up, w.w * up);
+                        const float4 x = widened(w[k], a.dtype);
+                        const float4 v = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
                         const uint2 hi = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
                         sm.q[slot][(k * NB + nb) * 32 + lane] = hi;
                         if constexpr (SPLIT) {
@@ -539,11 +563,11 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                             const int r = r0 + c;
                             if (r >= x.rows) continue;
                             if (whole) {
-                                const int row = x.row0 + r, h = x.hk * p.G + row % p.G;
+                                const int row = x.row0 + r, token = p.div(row), h = x.hk * p.G + row - token * p.G;
                                 const float inv = ml[c].y == 0.f ? 0.f : 1.f / ml[c].y;
 #pragma unroll
                                 for (int q = 0; q < 2 * JS; ++q) y[c][q] *= inv;
-                                store_out<2 * JS>(a, static_cast<long>(x.q0 + row / p.G) * a.ld_o + h * D + VB * g + 2 * j0, y[c]);
+                                store_out<2 * JS>(a, static_cast<long>(x.q0 + token) * a.ld_o + h * D + VB * g + 2 * j0, y[c]);
                             } else {
                                 float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<long>(slot) * MR + r) * D + VB * g + 2 * j0);
 #pragma unroll
@@ -557,8 +581,8 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                         const int r = r0 + c;
                         if (g != 0 || r >= x.rows) continue;
                         if (whole) {
-                            const int row = x.row0 + r, h = x.hk * p.G + row % p.G;
-                            a.lse[static_cast<long>(h) * b.N + x.q0 + row / p.G] =
+                            const int row = x.row0 + r, token = p.div(row), h = x.hk * p.G + row - token * p.G;
+                            a.lse[static_cast<long>(h) * b.N + x.q0 + token] =
                                 ml[c].y == 0.f ? -INFINITY : (ml[c].x + log2f(ml[c].y)) * kLn2;
                         } else {
                             p.part_ml[static_cast<long>(slot) * MR + r] = ml[c];
@@ -680,23 +704,29 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) s[gr][nb][2 * u + c] *= k_s * f[nb][c];
-                        if (!seen_all) {
-                            const int pos = pos0 + r, j = pos - base;  // j: the place among the new tokens
-                            const bool exists = pos < len && ((here >> gr) & 1);
-                            if (!exists) vs[gr][u] = 0.f;
+                        if (!seen_all && !(pos0 + r < len && ((here >> gr) & 1))) vs[gr][u] = 0.f;  // no such position
+                        raise |= vs[gr][u] > unit;
+                    }
+                if (!seen_all) {
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    const int mine = 8 * nb + 2 * t + c, token = (row0 + mine) / p.G;
-                                    bool see = exists && mine < rows;
-                                    if (see && j >= 0)
-                                        see = a.tree ? j < 64 && ((__ldg(a.tree + q0 + token) >> j) & 1) : j <= token;
+                        for (int c = 0; c < 2; ++c) {
+                            const int mine = 8 * nb + 2 * t + c, token = p.div(row0 + mine);
+                            // The new tokens that the row sees: a tree's, or all up to its own.
+                            unsigned long long bits = 0;
+                            if (a.tree && mine < rows && pos0 + 16 * GR > base) bits = __ldg(a.tree + q0 + token);
+#pragma unroll
+                            for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) {
+                                    const int pos = pos0 + 16 * gr + 8 * u + tau<D>(g), j = pos - base;
+                                    const bool see = mine < rows && pos < len && ((here >> gr) & 1) &&
+                                                     (j < 0 || (a.tree ? j < 64 && ((bits >> j) & 1) : j <= token));
                                     if (!see) s[gr][nb][2 * u + c] = -INFINITY;
                                 }
                         }
-                        raise |= vs[gr][u] > unit;
-                    }
+                }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -988,6 +1018,7 @@ ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, 
     p.a = a;
     p.page_shift = page_shift_of(b.c.page_size);
     p.G = a.H / b.c.n_kv_head;
+    p.inv_g = 0xFFFFFFFFu / p.G;
     // Row tiles of 8, 16 or 32, the smallest that holds a sequence's rows on average: fewer row tiles read
     // the cache less often, smaller ones leave fewer idle rows.  (350 MB read for one row tile of
     // 8, 16, 32 rows: 75, 103 and 188 us when the rule was set; four tiles of 8 would read it four times.)
