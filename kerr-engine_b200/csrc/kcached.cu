@@ -11,7 +11,7 @@
 // MMA operands with few instructions.  64 bf16 sequences' one token over up to 8191
 // positions, 8 key heads of 128, int8 codes, 347 MB: 86 us, 4.0 TB/s.  With more rows
 // the products' instructions bound it: trees of 8 tokens, 32 rows a key head, of two
-// sequences of up to 131k positions, 370 MB of e4m3: 143 us, 160 TFLOP/s.
+// sequences of up to 131k positions, 370 MB of e4m3: 130 us, 175 TFLOP/s.
 //
 // Rows.  The G query heads of a key head share its positions: a sequence's n
 // tokens are n * G rows, in row tiles of 8 * NB.  Positions are the m of
@@ -22,7 +22,8 @@
 // are one line of work, cut into as many equal parts as there are CTAs
 // (two to an SM), whatever the lengths; an item cut by a border leaves parts
 // (row maxima, sums, O) in a workspace, which cached_join adds in order.  An item
-// counts as EXTRA tiles more than it has: 98, 88 and 91 us for 0, 1 and 2 (the 64 sequences).
+// counts as EXTRA tiles more than it has: 85, 88 and 91 us for 1, 2 and 3 (the 64 sequences), 98
+// and 88 for 0 and 1 when the line came in.
 //
 // Operands.  Codes are exact in f16, so
 // only q and the weights are rounded: q to f16 after a power of two per row has

@@ -845,8 +845,11 @@ def _pages(cache, cu, kv_len, table, device):
     ld, inner = table.stride()
     if pages > 1 and inner != 1:
         raise ValueError("table must have unit inner stride")
-    return (_ints(cu, "cu", S + 1, device), _ints(kv_len, "kv_len", S, device), table.data_ptr(),
-            ld if ld > pages else pages, pages), S
+    if S < 2:
+        ld = pages
+    elif ld < pages:
+        raise ValueError("table's rows overlap")
+    return (_ints(cu, "cu", S + 1, device), _ints(kv_len, "kv_len", S, device), table.data_ptr(), ld, pages), S
 
 
 def fwd_packed(ctx: Context, q, k, v, o, lse, cu_q, cu_k, n_head: int, n_kv_head: int | None = None,

@@ -135,6 +135,16 @@ def test_binding_refusals():
                       (lambda: kerr_attn._sums(torch.zeros(4, 1), 1, 4, -1), ValueError)):
         with pytest.raises(kind):
             bad()
+    # A page table whose rows are one row, broadcast.
+    class Cache:
+        device_index = -1
+
+    row, lengths = torch.zeros(1, 5, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="overlap"):
+        kerr_attn._pages(Cache, torch.zeros(4, dtype=torch.int32), lengths, row.expand(3, 5), -1)
+    wide = torch.zeros(3, 9, dtype=torch.int32)
+    assert kerr_attn._pages(Cache, torch.zeros(4, dtype=torch.int32), lengths, wide[:, :5], -1)[0][3:] == (9, 5)
+    assert kerr_attn._pages(Cache, i, lengths[:1], row, -1)[0][3:] == (5, 5)
     assert kerr_attn._packed(x, "k", x.dtype, -1, -1, 64) == 64
     assert kerr_attn._packed(x[:, :32], "k", x.dtype, -1, 4, 32) == 64
     assert kerr_attn._packed(x[:1, :32], "k", x.dtype, -1, 1, 32) == 64
