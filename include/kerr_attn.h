@@ -412,7 +412,8 @@ int kattn_block_bwd(kattn_ctx* ctx, kattn_block* blk, const float* dh_out, float
  *
  * Types.  dtype names the element type of q, k, v and o: scores, softmax
  * statistics and sums are formed in f32, and outputs are rounded once.  Products
- * of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about 1e-6,
+ * of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about 1e-6
+ * (2e-6 at d = 128 over thousands of keys; a product in f32 is off by 1e-6 there),
  * with 2^-37 of the largest magnitude among a sequence's rows as the least step.
  * Sums of v are formed before they are divided: |v| is to stay below 2^96.
  * Device pointers are 16-byte aligned and row strides a multiple of 16 bytes;

@@ -38,7 +38,8 @@
 // them near 2^14: one a row of Q, one a tile of K, one for the V tiles of an item (it
 // rises when one needs it, and O follows).  They go back in with the exponent's factor
 // and the output.  bf16 pairs need no powers and took 84 us where this takes 94 (chunks
-// over cached contexts, f32), but are off by 6e-6; these by 3e-7 to 9e-7, as an f32 product is.
+// over cached contexts, f32), but are off by 6e-6; these by 3e-7 to 9e-7, as an f32 product is, and by up to 1.8e-6 at
+// D = 128, where TMEM has no room for a second O and every product is cut into the one sum.
 //
 // Weights are 2^(c s - c mu), c = scale log2(e), with mu raised only when a
 // tile's maximum passes it by more than 2^8 (then O and the sum are scaled): weights
@@ -67,8 +68,8 @@ constexpr int N_THREADS = 512, LAUNCH_REGS = 128;
 constexpr int LOAD_WARP = 8, MMA_WARP = 12, TMA_WARP = 13, ITEM_WARP = 14;
 constexpr int ITEMS = 4;         // item ring
 constexpr float RESCALE_LOG2 = 8.f;
-constexpr int UNITS = 16;       // ring of the K and V tiles' powers of two: more than tiles can be under way
-constexpr int POLY = 1;          // of 8 pairs of weights by the FMA units (16-bit types)
+constexpr int UNITS = 16;        // ring of the K and V tiles' powers of two: more than tiles can be under way
+constexpr int POLY = 1;          // of 8 pairs of weights by the FMA units (16-bit types): 582, 576, 586 us for 0, 1, 2 (long prompts)
 constexpr uint32_t TMEM_COLS = 512;
 constexpr size_t SMEM_MAX = 227 * 1024;
 
