@@ -456,15 +456,17 @@ struct LineWalker {
         if (t0 > 0 && t1 == all && (threadIdx.x & 31) == 0)
             p.joins[cta] = Join{first_cta, it.q0, it.nq, it.hk, it.r0};
         at = Border{at.item + 1, 0};
-        if (++i == tiles && (at.item < to.item || (at.item == to.item && to.tile > 0))) {
-            i = 0;
-            int y = s + 1;
-            if (at.item % head_items == 0) {
-                ++hk;
-                y = 0;
+        ++i;
+        if (at.item < to.item || (at.item == to.item && to.tile > 0)) {
+            // A key head's items end by their number: offsets that descend may make more than the plan took, and
+            // its last item then lies inside a sequence.  Before it, a sequence with items follows.
+            const bool head_end = at.item % head_items == 0;
+            if (head_end || i == tiles) {
+                hk += head_end ? 1 : 0;
+                i = 0;
+                load(head_end ? 0 : s + 1);
+                while (tiles == 0 && s + 1 < p.a.S) load(s + 1);
             }
-            load(y);
-            while (tiles == 0) load(s + 1);
         }
         return it;
     }
