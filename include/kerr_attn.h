@@ -118,10 +118,10 @@ int kattn_set_wait_limit(kattn_ctx* ctx, unsigned long long ns);
 int kattn_set_deterministic(kattn_ctx* ctx, int on);
 
 /* Diagnostic for the bounded waits: the next tensor-core forward launched on
- * this context issues no copy of its first key tile, so the waits on that
- * tile run out after the wait limit and the kernel unwinds as above (its
- * outputs are undefined).  Later calls run normally.  For tests of the
- * timeout path; no counterpart in the reference. */
+ * this context (kattn_fwd, kattn_fwd_packed or kattn_fwd_cached) issues no copy
+ * of its first key tile, so the waits on that tile run out after the wait limit
+ * and the kernel unwinds as above (its outputs are undefined).  Later calls run
+ * normally.  For tests of the timeout path; no counterpart in the reference. */
 int kattn_test_withhold_next_load(kattn_ctx* ctx);
 
 /* Waits for the context's device to finish its work and reports whether any

@@ -184,6 +184,7 @@ struct PackedArgs {
     int causal;
     int* status = nullptr;
     unsigned long long wait_ns = 1000000000ull;
+    int withhold_first_key_load = 0;  // diagnostic (kattn_test_withhold_next_load): each CTA's first key tile never lands
 };
 ProjStatus packed_forward(const PackedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
 
@@ -215,6 +216,7 @@ struct CachedArgs {
     float scale;
     int* status = nullptr;
     unsigned long long wait_ns = 1000000000ull;
+    int withhold_first_key_load = 0;  // as PackedArgs's
 };
 ProjStatus cached_forward(const CachedArgs& a, int num_sms, cudaMemPool_t pool, cudaStream_t s, int* launches);
 

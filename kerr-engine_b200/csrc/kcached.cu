@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                         mbar_arrive_expect_tx(&sm.full[st], __popc(there) * 2 * frag * D);
                     }
                     __syncwarp();
-                    if (page >= 0) {
+                    if (page >= 0 && !(a.withhold_first_key_load && i == 0 && j == x.t0)) {
                         const int row = (x.hk << p.page_shift) + ((j * TK + lane * frag) & (b.c.page_size - 1));
                         tma_load_3d(sm.k[st] + lane * frag * D, &p.tk, 0, row, page, &sm.full[st]);
                         tma_load_3d(sm.v[st] + lane * frag * D, &p.tv, 0, row, page, &sm.full[st]);

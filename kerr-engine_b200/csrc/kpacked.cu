@@ -1057,6 +1057,9 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                             mma_commit_elected(&sm.o_full[t], one);
                         }
                     }
+                    // After a wait that ran out no stage goes back: its copy may still be on its way, and a second
+                    // copy's arrival in the same phase of its barrier would be one too many.
+                    if (failed) break;
                     if (j > 0) {
                         mma_commit_elected(&sm.kv_empty[st], one);
                         if (++st == C::STAGES) st = 0, phase ^= 1;
@@ -1102,7 +1105,8 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                         mbar_arrive_expect_tx(bar, C::KV_BYTES);
 #pragma unroll
                         for (int b = 0; b < C::BLOCKS; ++b)
-                            tma_load_2d(sm.kv[st] + b * C::KV_BLOCK, map, it.hk * D + 64 * b, it.k0 + j * BN, bar);
+                            if (kv != 0 || !p.a.withhold_first_key_load)
+                                tma_load_2d(sm.kv[st] + b * C::KV_BLOCK, map, it.hk * D + 64 * b, it.k0 + j * BN, bar);
                     }
                     if (tail) {
                         if (!mbar_wait_warp(&sm.tail, tails++ & 1, limit)) {

@@ -141,7 +141,8 @@ int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const 
     DeviceScope scope(ctx->device);
     if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
     const kattn::PackedArgs a{dtype, q,  ld_q, k, v, ld_kv, o, ld_o, lse, cu_q, cu_k, S, Nq, Nk, H, Hkv, d,
-                              scale, causal, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed)};
+                              scale, causal, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed),
+                              ctx->withhold_next_load.exchange(0)};
     int launches = 0;
     const kattn::ProjStatus st =
         kattn::packed_forward(a, ctx->num_sms, ctx->pool, static_cast<cudaStream_t>(stream), &launches);
@@ -199,7 +200,8 @@ int kattn_fwd_cached(kattn_ctx* ctx, const kattn_kv_cache* cache, int dtype, con
     DeviceScope scope(ctx->device);
     if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
     const kattn::CachedArgs a{{*cache, cu, kv_len, table, ld_table, max_pages, S, N}, dtype, q, ld_q, o, ld_o, lse,
-                              tree, H, scale, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed)};
+                              tree, H, scale, ctx->d_status, ctx->wait_ns.load(std::memory_order_relaxed),
+                              ctx->withhold_next_load.exchange(0)};
     int launches = 0;
     const kattn::ProjStatus st =
         kattn::cached_forward(a, ctx->num_sms, ctx->pool, static_cast<cudaStream_t>(stream), &launches);

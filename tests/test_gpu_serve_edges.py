@@ -7,7 +7,7 @@ import torch
 
 import kerr_attn
 import serve_ref
-from test_gpu_serve import ints, randn
+from test_gpu_serve import fill, ints, make_cache, offsets, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,76 @@ def test_packed_plan_ends_inside_a_sequence(ctx):
     want, wl, bo, bl = serve_ref.packed(q[:M], k[:M], v[:M], [0, M], [0, M], H, Hkv, True, 1 / math.sqrt(d))
     serve_ref.check(o[:M], want, bo, "o")
     serve_ref.check(lse[:, :M], wl, bl, "lse")
+
+
+def check_withheld(call, limit_ns):
+    """call(ctx) with a copy withheld: the waits run out after the limit, the call ends with the status word set,
+    and the same context then gives the same bits as before."""
+    with kerr_attn.Context(0) as ctx:
+        usual = [x.clone() for x in call(ctx)]
+        ctx.check_device()
+        for _ in range(3):
+            ctx.set_wait_limit(limit_ns)
+            ctx.test_withhold_next_load()
+            call(ctx)
+            with pytest.raises(kerr_attn.KattnError) as e:
+                ctx.check_device()
+            assert e.value.status == kerr_attn.KATTN_ERR_DEVICE_TIMEOUT
+            ctx.check_device()  # the report cleared the flag
+            ctx.set_wait_limit(0)
+            again = call(ctx)
+            ctx.check_device()
+            assert all(torch.equal(a, b) for a, b in zip(usual, again))
+
+
+def packed_call(dtype, d, whole):
+    gen = torch.Generator().manual_seed(41)
+    nq, H, Hkv = [300, 1, 777, 40, 1200], 32 if whole else 8, 16 if whole else 4
+    nk = nq if whole else [900, 2, 4777, 1600, 1200]
+    q = randn(gen, sum(nq), H * d, dtype=dtype)
+    k, v = (randn(gen, sum(nk), Hkv * d, dtype=dtype) for _ in range(2))
+    cu_q, cu_k = ints(offsets(nq)), ints(offsets(nk))
+    o, lse = torch.empty_like(q), torch.empty(H, q.shape[0], device="cuda")
+
+    def call(ctx):
+        # Whole items, or parts and a join.
+        assert kerr_attn.fwd_packed(ctx, q, k, v, o, lse, cu_q, cu_k, H, Hkv) == (1 if whole else 2)
+        return o, lse
+
+    return call
+
+
+def cached_call(dtype, d, fmt, rows):
+    gen = torch.Generator().manual_seed(42)
+    kv_len, new, Hkv = [5000, 300, 9000, 40], [rows, 1, 1, rows], 8
+    cache, table = make_cache(kv_len, 32, Hkv, d, fmt, seed=43)
+    with kerr_attn.Context(0) as ctx:
+        fill(ctx, cache, table, kv_len, dtype, seed=44)
+    H = 2 * Hkv
+    q = randn(gen, sum(new), H * d, dtype=dtype)
+    cu, lengths = ints(offsets(new)), ints(kv_len)
+    o, lse = torch.empty_like(q), torch.empty(H, q.shape[0], device="cuda")
+
+    def call(ctx):
+        kerr_attn.fwd_cached(ctx, cache, q, o, lse, cu, lengths, table, H)
+        return o, lse
+
+    return call
+
+
+MS = 1_000_000
+
+
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_withheld_copy(dtype, d, whole):
+    check_withheld(packed_call(dtype, d, whole), MS)
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("fmt", [kerr_attn.CACHE_INT8, kerr_attn.CACHE_E4M3])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cached_withheld_copy(dtype, d, fmt, rows):
+    check_withheld(cached_call(dtype, d, fmt, rows), MS)
