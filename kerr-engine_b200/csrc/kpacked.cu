@@ -68,6 +68,7 @@ constexpr int N_THREADS = 512, LAUNCH_REGS = 128;
 constexpr int LOAD_WARP = 8, MMA_WARP = 12, TMA_WARP = 13, ITEM_WARP = 14;
 constexpr int ITEMS = 4;         // item ring
 constexpr float RESCALE_LOG2 = 8.f;
+constexpr uint32_t GAVE_UP = 0xFFFFFFFFu;  // for a largest magnitude's bits: the warp's wait ran out
 constexpr int UNITS = 16;        // ring of the K and V tiles' powers of two: more than tiles can be under way
 constexpr int POLY = 1;          // of 8 pairs of weights by the FMA units (16-bit types): 582, 576, 586 us for 0, 1, 2 (long prompts)
 constexpr uint32_t TMEM_COLS = 512;
@@ -92,7 +93,7 @@ struct Cfg {
     static constexpr bool BF16 = std::is_same_v<T, __nv_bfloat16>;  // the operands' type; else f16
     static constexpr float W_UP = SPLIT ? 7.f : 0.f;  // weights are held times 2^7 (then at most 2^15), far from f16's subnormals
     // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
-    static constexpr int R_SOFT = SPLIT ? 184 : 200, R_LOAD = SPLIT ? 96 : 64, R_SERV = 48;
+    static constexpr int R_SOFT = SPLIT ? 176 : 200, R_LOAD = SPLIT ? 112 : 64, R_SERV = 48;
     static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 4 * LAUNCH_REGS, "register split");
     __host__ __device__ static constexpr uint32_t col_s(int t) { return t * BN; }
     // Pairs at D <= 64: V's hi and lo are one operand of 2 D columns, and O two halves that are added at the end.  An MMA
@@ -978,14 +979,16 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     const bool ok = mbar_wait_busy(&sm.raw_full[st], (kv / C::STAGES) & 1, limit);
                     F32Tile<D> tile;
                     tile.read(sm.kv[st], it.nk - it.shift - (x >> 1) * BN, lt);
-                    const uint32_t own = __reduce_max_sync(0xffffffffu, tile.most());
+                    const uint32_t own = __reduce_max_sync(0xffffffffu, ok ? tile.most() : GAVE_UP);
                     if (lane == 0) sm.most[kv & 1][warp - LOAD_WARP] = own;
-                    if (named_sync_or(1, 128, !ok || failed)) {
+                    named_sync(1, 128);
+                    const uint32_t* w = sm.most[kv & 1];
+                    const uint32_t most = max(max(w[0], w[1]), max(w[2], w[3]));
+                    if (most == GAVE_UP) {
                         failed = true;
                         break;
                     }
-                    const uint32_t* w = sm.most[kv & 1];
-                    float unit = unit_2_14(max(max(w[0], w[1]), max(w[2], w[3])));
+                    float unit = unit_2_14(most);
                     if (x & 1) unit = unit_v = x == 1 || unit > unit_v ? 4.f * unit : unit_v;
                     if (lt == 0) sm.unit_kv[kv % UNITS] = unit;
                     tile.write(sm.kv[st], inverse_of_power(unit), lt);
@@ -1152,7 +1155,15 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
             }
         }
     }
-    if (failed && lane == 0) atomicOr(p.a.status, 1);
+    if (failed) {
+        if (lane == 0) atomicOr(p.a.status, 1);
+        if (C::SPLIT && warp >= LOAD_WARP && warp < MMA_WARP) {
+            // The loaders meet at every tile: one whose wait ran out elsewhere lets the others out of their next meeting.
+            if (lane < 2) sm.most[lane][warp - LOAD_WARP] = GAVE_UP;
+            __syncwarp();
+            named_arrive(1, 128);
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

@@ -176,6 +176,11 @@ __device__ __forceinline__ void named_sync(uint32_t id, uint32_t nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// The same without waiting, for a warp that others meet and that goes its own way.
+__device__ __forceinline__ void named_arrive(uint32_t id, uint32_t nthreads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
 // Named barrier that also returns whether `pred` held on any participating thread.
 __device__ __forceinline__ bool named_sync_or(uint32_t id, uint32_t nthreads, bool pred) {
     uint32_t r;

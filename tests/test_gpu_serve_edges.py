@@ -110,3 +110,10 @@ def test_packed_withheld_copy(dtype, d, whole):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_cached_withheld_copy(dtype, d, fmt, rows):
     check_withheld(cached_call(dtype, d, fmt, rows), MS)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_packed_withheld_copy_f32(d, whole):
+    # The four warps that convert f32 tiles meet at every tile: all of them leave when one gives up.
+    check_withheld(packed_call(torch.float32, d, whole), MS)
