@@ -1125,13 +1125,13 @@ __global__ void __launch_bounds__(N_THREADS, 1) packed_fwd(const __grid_constant
                     }
                 }
             }
-            if (failed) {
-                // Copies still landing complete before the shared memory is released.
-                for (int x = max(0, kv - C::STAGES); x < kv; ++x)
-                    mbar_wait(C::SPLIT ? &sm.raw_full[x % C::STAGES] : &sm.kv_full[x % C::STAGES], (x / C::STAGES) & 1,
-                              10000000ull);
-                if (tails > 0) mbar_wait(&sm.tail, (tails - 1) & 1, 10000000ull);
-            }
+            // Copies still landing complete before the shared memory is released, also where it is another warp that gave
+            // up (elsewhere the last tiles are waited for in any case).
+#pragma unroll 1
+            for (int x = max(0, kv - C::STAGES); x < kv; ++x)
+                mbar_wait(C::SPLIT ? &sm.raw_full[x % C::STAGES] : &sm.kv_full[x % C::STAGES], (x / C::STAGES) & 1,
+                          10000000ull);
+            if (failed && tails > 0) mbar_wait(&sm.tail, (tails - 1) & 1, 10000000ull);
         } else if (warp == ITEM_WARP) {
             // -------------------------------------------------------- items
             const int ctas = gridDim.x, b = blockIdx.x;

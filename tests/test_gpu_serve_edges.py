@@ -117,3 +117,12 @@ def test_cached_withheld_copy(dtype, d, fmt, rows):
 def test_packed_withheld_copy_f32(d, whole):
     # The four warps that convert f32 tiles meet at every tile: all of them leave when one gives up.
     check_withheld(packed_call(torch.float32, d, whole), MS)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_packed_gives_up_with_copies_in_flight(dtype, d, whole):
+    # Waits run out at their first look, each warp where it happens to be, while the copies behind the withheld one are
+    # on their way: they land before the shared memory is released.
+    check_withheld(packed_call(dtype, d, whole), 1)
