@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                     sm.pieces[i % PIECES] = x;
                     mbar_arrive(&sm.piece_full[i % PIECES]);
                 }
-                if (!more) return;
+                if (!more) break;
                 // Lane f looks up the page of the f-th stretch, a tile ahead.
                 auto page_at = [&](int tile) {
                     const int pos = tile * TK + lane * frag;
@@ -477,7 +477,8 @@ __global__ void __launch_bounds__(N_THREADS, 2) cached_fwd(const __grid_constant
                 }
                 if (!ok) break;
             }
-            // After a wait that ran out: copies still landing complete before the shared memory is released.
+            // Copies still landing complete before the shared memory is released, also where it is another warp that gave
+            // up (elsewhere they are waited for in any case).
             for (int f = 0; f < C::STAGES; ++f) {
                 if (turn > 0) mbar_wait(&sm.full[st], (turn - 1) & 1, 10000000ull);
                 if (++st == C::STAGES) st = 0, ++turn;

@@ -126,3 +126,10 @@ def test_packed_gives_up_with_copies_in_flight(dtype, d, whole):
     # Waits run out at their first look, each warp where it happens to be, while the copies behind the withheld one are
     # on their way: they land before the shared memory is released.
     check_withheld(packed_call(dtype, d, whole), 1)
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cached_gives_up_with_copies_in_flight(dtype, d, rows):
+    check_withheld(cached_call(dtype, d, kerr_attn.CACHE_INT8, rows), 1)
