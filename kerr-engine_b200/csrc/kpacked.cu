@@ -43,7 +43,7 @@
 //
 // Weights are 2^(c s - c mu), c = scale log2(e), with mu raised only when a
 // tile's maximum passes it by more than 2^8 (then O and the sum are scaled): weights
-// stay below 2^8, which f16 holds, and O is almost never read back.
+// stay below 2^8 (2^15 as f16 holds them), and O is almost never read back.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -91,7 +91,9 @@ struct Cfg {
     static constexpr int FIT = static_cast<int>((SMEM_MAX - 2048 - OUT_BYTES - 2 * Q_BYTES) / KV_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;  // K and V tiles in flight
     static constexpr bool BF16 = std::is_same_v<T, __nv_bfloat16>;  // the operands' type; else f16
-    static constexpr float W_UP = SPLIT ? 7.f : 0.f;  // weights are held times 2^7 (then at most 2^15), far from f16's subnormals
+    // f16 weights are held times 2^7 (then at most 2^15), further from f16's subnormals: a weight of 2^-25 of the largest
+    // and less would vanish, and tens of thousands of those are more than the output's rounding.
+    static constexpr float W_UP = BF16 ? 0.f : 7.f;
     // Registers of a softmax, loader and service thread (LAUNCH_REGS at launch).
     static constexpr int R_SOFT = SPLIT ? 176 : 200, R_LOAD = SPLIT ? 112 : 64, R_SERV = 48;
     static_assert(2 * R_SOFT + R_LOAD + R_SERV <= 4 * LAUNCH_REGS, "register split");

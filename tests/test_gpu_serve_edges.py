@@ -133,3 +133,27 @@ def test_packed_gives_up_with_copies_in_flight(dtype, d, whole):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_cached_gives_up_with_copies_in_flight(dtype, d, rows):
     check_withheld(cached_call(dtype, d, kerr_attn.CACHE_INT8, rows), 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_packed_many_small_weights(ctx, dtype):
+    # One key takes nearly all of the weight and has a value of zero: the output is 60000 others', each 2^-26 of it.
+    # As many rows as whole items take, so that every item sees all keys; all rows are alike.
+    d, rows, n = 64, 115200, 60000
+    q = torch.zeros(rows, d, dtype=dtype, device="cuda")
+    q[:, 0] = 4.0
+    k = torch.zeros(n + 1, d, dtype=dtype, device="cuda")
+    k[1:, 0] = -4.5
+    v = torch.rand(n + 1, d, generator=torch.Generator().manual_seed(45)).add(0.5).to(dtype).cuda()
+    v[0] = 0
+    o, lse = torch.empty_like(q), torch.empty(1, rows, device="cuda")
+    assert kerr_attn.fwd_packed(ctx, q, k, v, o, lse, ints([0, rows]), ints([0, n + 1]), 1, 1, causal=False, scale=1.0) == 1
+    w = math.exp(-18.0)
+    want = w * v[1:].double().sum(0) / (1 + n * w)
+    # A weight, held times 2^7, is off by 2^-25 where f16 is subnormal, else by u of itself; the output by u; the score by
+    # its product's f32 sums and exp2's 2^-21; O's sums of 16 keys at a time, and l's of 128, by an f32 step each.
+    u = serve_ref.U[dtype]
+    relative = 2 * u + 2 * ((d + 3) * 2.0 ** -24 * 18 + 2.0 ** -21) + (n / 16) * 2.0 ** -23 + (n / 128) * 2.0 ** -24
+    bound = n * 2.0 ** -32 * v.double().max() + relative * want
+    assert ((o.double() - want).abs() <= bound).all()
+    assert (lse - math.log1p(n * w)).abs().max() <= 2.0 ** -20 + (n / 128) * 2.0 ** -24
