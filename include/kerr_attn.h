@@ -411,11 +411,16 @@ int kattn_block_bwd(kattn_ctx* ctx, kattn_block* blk, const float* dh_out, float
  * never synchronise the host.
  *
  * Types.  dtype names the element type of q, k, v and o: scores, softmax
- * statistics and sums are formed in f32, and outputs are rounded once.  Products
- * of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about 1e-6
- * (2e-6 at d = 128 over thousands of keys; a product in f32 is off by 1e-6 there),
- * with 2^-37 of the largest magnitude among a sequence's rows as the least step.
- * Sums of v are formed before they are divided: |v| is to stay below 2^96.
+ * statistics and sums are formed in f32, and outputs are rounded once.  Weights
+ * meet v rounded to the type (kattn_fwd_cached: to f16, for KATTN_BF16 too).
+ * Products of KATTN_F32 are of f16 hi/lo pairs behind powers of two: 22 bits, about
+ * 1e-6 (2e-6 at d = 128 over thousands of keys; a product in f32 is off by 1e-6
+ * there), with 2^-37 of the largest magnitude among a sequence's rows as the least
+ * step.  Over a cache a position's share of an output has 2^-31 of the largest
+ * |v| among the sequence's positions as its least step, of every type and also for
+ * rows that do not see that position: weights are held times the values' scales.
+ * Sums of v are formed before they are divided: |v| is to stay below 2^96, and d
+ * times the largest |q| times the largest |k| below 2^127.
  * Device pointers are 16-byte aligned and row strides a multiple of 16 bytes;
  * int32 arrays and lse 4-byte, tree 8-byte aligned.  d is 32, 64 or 128.
  *

@@ -30,6 +30,9 @@
 // brought its largest element near 2^13 (exact for bf16 and f16 but for elements 2^-37
 // of it; f32 as a hi / lo pair), the weights p_j vs_j to f16 after a power of two
 // per warp (f32: as a pair).  The scale ks_j multiplies the score.
+// A weight's step is 2^-24 (f16's subnormals, a pair's too) where its largest, by the power of two, is 2^7 for
+// a row's first score: with codes up to the limit L and that power at most twice the largest scale, a position
+// is off by 2^-25 2^-7 2 max|v| = 2^-31 max|v| at most, whoever sees the largest.
 //
 // Lanes read whole 16-byte chunks of codes: the order of d in the first product
 // is free (q is permuted alike), and in the second a lane's chunk spreads over

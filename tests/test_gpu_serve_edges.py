@@ -157,3 +157,32 @@ def test_packed_many_small_weights(ctx, dtype):
     bound = n * 2.0 ** -32 * v.double().max() + relative * want
     assert ((o.double() - want).abs() <= bound).all()
     assert (lse - math.log1p(n * w)).abs().max() <= 2.0 ** -20 + (n / 128) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("power", [0, 10, 20, 30])
+@pytest.mark.parametrize("fmt", [kerr_attn.CACHE_INT8, kerr_attn.CACHE_E4M3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_cached_beside_a_far_larger_value(ctx, dtype, fmt, power):
+    # A drafted token whose values are 2^power times the others', which only the second row sees: the first row's
+    # positions are off by 2^-31 of the largest value each, besides the usual bounds.
+    gen = torch.Generator().manual_seed(46)
+    H, Hkv, d, length = 4, 2, 64, 6
+    cache, table = make_cache([length], 16, Hkv, d, fmt, seed=47)
+    k, v = randn(gen, length, Hkv * d), randn(gen, length, Hkv * d)
+    v[length - 1] *= 2.0 ** power
+    kerr_attn.cache_append(ctx, cache, k, v, ints([0, length]), ints([length]), table)
+    q = randn(gen, 2, H * d, dtype=dtype)
+    o, lse = torch.empty_like(q), torch.empty(H, 2, device="cuda")
+    kerr_attn.fwd_cached(ctx, cache, q, o, lse, ints([0, 2]), ints([length]), table, H, tree=torch.tensor([1, 3]).cuda())
+    kc, vc = serve_ref.values(cache)
+    page = int(table[0, 0])
+    held = [(c * s.cpu().double()[..., None])[page].transpose(0, 1) for c, s in ((kc, cache.k_scale), (vc, cache.v_scale))]
+    for row, n in ((0, length - 1), (1, length)):
+        want, wl, bo, bl = serve_ref.attend(q[row:row + 1].cpu().double().view(1, H, d), held[0][:n], held[1][:n],
+                                            torch.ones(1, n, dtype=torch.bool), 1 / math.sqrt(d), dtype)
+        bo = bo + n * 2.0 ** -31 * held[1].abs().max()
+        if dtype == torch.float16:  # from 65520 on the nearest f16 is an infinity; within the bound of it either is right
+            want = torch.where(want.abs() - bo > 65520, want * math.inf, want)
+            want = torch.where((want.abs() - 65520).abs() <= bo, math.nan, want)
+        serve_ref.check(o[row:row + 1].view(1, H, d), want, bo, f"o of row {row}")
+        serve_ref.check(lse[:, row:row + 1], wl, bl, f"lse of row {row}")
