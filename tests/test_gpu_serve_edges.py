@@ -186,3 +186,45 @@ def test_cached_beside_a_far_larger_value(ctx, dtype, fmt, power):
             want = torch.where((want.abs() - 65520).abs() <= bo, math.nan, want)
         serve_ref.check(o[row:row + 1].view(1, H, d), want, bo, f"o of row {row}")
         serve_ref.check(lse[:, row:row + 1], wl, bl, f"lse of row {row}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cached_shared_pages(ctx, dtype):
+    # Two sequences whose earlier positions lie on the same pages, and one that has a page twice.
+    H, Hkv, d, page = 4, 2, 64, 16
+    cache, _ = make_cache([160], page, Hkv, d, kerr_attn.CACHE_INT8, seed=48)
+    table = ints([[3, 5, 1, 7], [3, 5, 2, 0], [4, 4, 6, 0]])
+    gen = torch.Generator().manual_seed(49)
+    cu, kv_len = [0, 50, 53, 56], [50, 35, 40]
+    k, v = randn(gen, 56, Hkv * d, dtype=dtype), randn(gen, 56, Hkv * d, dtype=dtype)
+    for s in range(3):  # one after the other: the third's pages hold what is on them
+        kerr_attn.cache_append(ctx, cache, k[cu[s]:cu[s + 1]], v[cu[s]:cu[s + 1]], ints([0, cu[s + 1] - cu[s]]),
+                               ints(kv_len[s:s + 1]), table[s:s + 1])
+    q = randn(gen, 7, H * d, dtype=dtype)
+    o, lse = torch.empty_like(q), torch.empty(H, 7, device="cuda")
+    kerr_attn.fwd_cached(ctx, cache, q, o, lse, ints([0, 1, 4, 7]), ints(kv_len), table, H)
+    want, wl, bo, bl = serve_ref.cached(cache, q, [0, 1, 4, 7], kv_len, table, H, None, 1 / math.sqrt(d))
+    serve_ref.check(o, want, bo, "o")
+    serve_ref.check(lse, wl, bl, "lse")
+
+
+def test_cached_broken_offsets_and_lengths_stay_inside(ctx):
+    # Offsets that descend or leave the arrays, lengths below zero and past the table, pages that do not exist: every
+    # call keeps inside its arrays.
+    H, Hkv, d, N, page = 4, 2, 64, 100, 16
+    cu, kv_len = ints([0, 500, 40, -7, 1000, 60, 100]), ints([-5, 2 ** 31 - 1, 33, 90, 0, 64])
+    table = ints([[0, 9, -3, 2, 2 ** 31 - 1, 1]] * 6)
+    guard = torch.full((2, 6, Hkv, page, d), 5, dtype=torch.int8, device="cuda")
+    scales = torch.full((2, 6, Hkv, page), 3.0, device="cuda")
+    cache = kerr_attn.KVCache(guard[0, 1:4], guard[1, 1:4], scales[0, 1:4], scales[1, 1:4])  # pages amid others
+    wide = torch.full((4, N + 40, H * d), 3.0, device="cuda")
+    q, o, k, v = (x[20:20 + N] for x in wide)
+    lse = torch.zeros(H, N, device="cuda")
+    kv = [x[:, :Hkv * d] for x in (k, v)]
+    kerr_attn.cache_append(ctx, cache, *kv, cu, kv_len, table)
+    kerr_attn.cache_read(ctx, cache, *kv, cu, kv_len, table)
+    kerr_attn.fwd_cached(ctx, cache, q, o, lse, cu, kv_len, table, H)
+    ctx.check_device()
+    assert (wide[:, :20] == 3).all() and (wide[:, 20 + N:] == 3).all() and (wide[2:, :, Hkv * d:] == 3).all()
+    for x, value in ((guard, 5), (scales, 3)):
+        assert (x[:, 0] == value).all() and (x[:, 4:] == value).all()
