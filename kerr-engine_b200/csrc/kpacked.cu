@@ -14,12 +14,15 @@
 //
 // Work.  Where enough items share the GPU, each CTA takes whole ones, longest first.  A few long
 // ones are a line of key tiles cut into equal parts, one a CTA, and packed_join adds the
-// parts of cut items; line_pays() has the rule and what both measured.
+// parts of cut items; line_pays() has the rule and what both measured.  The search for a whole item
+// sweeps all sequences, so it grows with their square and from some hundreds on is what takes the time
+// (sequences of 64, 8 heads of 64, bf16: 53 us for 128 of them, 283 for 512, 13.6 ms for 4096).
 //
 // Bounds.  Long prompts: the tensor core's rate, shared with the exponentials (three bf16 prompts of
-// 1500 .. 8192, 32 heads of 128: 570 us, 1130 TFLOP/s; 660 us, 980 TFLOP/s from a cold L2).  f32: three products of each, whose
-// operands shared memory feeds, 3300 clocks a step.  Short prompts: the chain from launch to first copy
-// to store (one f32 prompt of 256, 12 heads: 19 us; 32 bf16 prompts of 9 .. 512, 20 heads on 4: 27 us).
+// 1500 .. 8192, 32 heads of 128: 580 us, 1110 TFLOP/s, back to back at 1965 MHz; 633 us after other work there; 660 us,
+// 980 TFLOP/s, once the power cap has brought the clock to 1.7 GHz).  f32: three products of each, whose operands shared
+// memory feeds, 3300 clocks a step.  Short prompts: the chain from launch to first copy
+// to store (one f32 prompt of 256, 12 heads: 19 us; 32 bf16 prompts of 9 .. 512, 20 heads on 4: 28 us).
 //
 // Warps (16).  0-3 and 4-7: the softmax of the first and the second row tile,
 // one thread a row.  8-11: Q into shared memory (and, for f32, K and V split
@@ -37,7 +40,7 @@
 // ones as f16 pairs (22 bits), hi*hi + hi*lo + lo*hi, after powers of two have brought
 // them near 2^14: one a row of Q, one a tile of K, one for the V tiles of an item (it
 // rises when one needs it, and O follows).  They go back in with the exponent's factor
-// and the output.  bf16 pairs need no powers and took 84 us where this takes 94 (chunks
+// and the output.  bf16 pairs need no powers and took 84 us where this took 94 (91 now; chunks
 // over cached contexts, f32), but are off by 6e-6; these by 3e-7 to 9e-7, as an f32 product is, and by up to 1.8e-6 at
 // D = 128, where TMEM has no room for a second O and every product is cut into the one sum.
 //
@@ -180,8 +183,7 @@ struct Params {
     float4* part_o;   // [2 * CTAs][D / 4][256 rows]: a CTA's part that began before it (0) or begins in it (1)
     float* part_lse;  // [2 * CTAs][256 rows]: log2 of the rows' sums
     Join* joins;      // [CTAs]
-    // x / G for x below 2^32 / G (the product is off by less than x G / 2^32).
-    // x / G: the product is at most one too large, and is from x = 2^32 / G on.
+    // x / G: x inv_g / 2^32 is too large by less than x / 2^32, which shows from x = 2^32 / G on, by one.
     __device__ __forceinline__ int div(int x) const {
         if (G == 1) return x;
         const uint32_t y = __umulhi(x, inv_g);
@@ -313,7 +315,8 @@ constexpr int ITEM_COST = 3, MIN_PART = 5;
 // and join cost what 5 steps do.  Dealt whole and in parts, us: one bf16 prompt of 1024 and of
 // 2048, 12 heads of 64, 20.6 and 23.4, 34.3 and 29.3; 16 of 512, 12 heads on 4, 29.2 and 37.5; 8 f32
 // chunks of 100 .. 1000 behind up to 3096 positions 112 and 94; three bf16 prompts of 1500 ..
-// 8192, 32 heads of 128 on 8, 576 and 644.
+// 8192, 32 heads of 128 on 8, 576 and 644 (when the rule was set).  It knows averages only: one prompt of 8192 is
+// 66 us in parts, but 124 us beside 31 of 64, whole (2 heads of 64).
 inline bool line_pays(const PackedArgs& a, long items, int num_sms) {
     const double nk = static_cast<double>(a.Nk) / a.S, nq = std::min(static_cast<double>(a.Nq) / a.S, nk);
     const double mean = items / static_cast<double>(num_sms) * (nk - (a.causal ? nq / 2 : 0)) / 128;
