@@ -433,7 +433,9 @@ enum { KATTN_F32 = 0, KATTN_BF16 = 1, KATTN_F16 = 2 };
  * sees all keys, the one before all but the last, and so on: row i sees keys j <=
  * i + nk - nq (every key when causal == 0).  So nk == nq is a prompt, nk > nq a
  * prompt's next chunk behind its earlier context (kattn_cache_read gives its
- * keys and values), and with nk < nq the first rows see nothing. */
+ * keys and values), and with nk < nq the first rows see nothing.  Any number of
+ * sequences is right, but from some hundreds on the call's time grows with their
+ * square: split larger batches over calls. */
 int kattn_fwd_packed(kattn_ctx* ctx, int dtype, const void* q, long ld_q, const void* k, const void* v, long ld_kv,
                      void* o, long ld_o, float* lse, const int* cu_q, const int* cu_k, int S, int Nq, int Nk, int H,
                      int Hkv, int d, float scale, int causal, void* stream);
